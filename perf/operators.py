@@ -285,7 +285,7 @@ def run(st):
         info = reorder(*cache, st["parents"], case["shift"], grow=st["grow"])
         return info, st["base_rows"], st["lens"], st["refs"], st["arrays"]
     left = reorder(*cache, st["leave"], case["shift"])
-    packed = compact(*cache, case["shift"])
+    packed = compact(st["arrays"], st["base_rows"], st["refs"], case["shift"])
     info = reorder(*cache, st["parents"], case["shift"], grow=st["grow"])
     st["lens"].add_(st["grow"])
     return left, packed, info, st["base_rows"], st["lens"], st["refs"], st["arrays"]
@@ -404,7 +404,7 @@ def _reorder(arrays, table, lens, refs, parents, shift, grow=None):
     return torch.stack([got.sum(), copied.sum(), fresh.sum() - got.sum(), zero]).to(torch.int32)
 
 
-def _compact(arrays, table, lens, refs, shift):
+def _compact(arrays, table, refs, shift):
     pages = refs.shape[0]
     at = torch.arange(pages, device=DEV)
     live = refs != 0
