@@ -520,6 +520,140 @@ int bq_full_attention(const int8_t* q_i8, const float* qi_bias, const float* f_q
                       int page_shift, int row_mask, int page_mask, int s_max, int seq_len,
                       void* stream);
 
+/* ---- paged 16-bit cache ------------------------------------------------------- */
+
+/* The operators below keep keys and values in bf16 (BQ_DT_BF16) or f16
+ * (BQ_DT_F16), [num_slots, num_kv * head_dim] each, in pages of
+ * 2^page_shift rows (page_shift 0 to 20).  The page table is base_rows
+ * [num_seqs, max_pages] int32: the first row of the page with a sequence's
+ * positions [j << page_shift, (j + 1) << page_shift), or -1.  It is
+ * bq_full_attention's base_rows too, with rows_off = sequence * max_pages,
+ * row_mask = 2^page_shift - 1 and page_mask = -1.  An entry whose page does not
+ * lie within the cache's rows counts as -1: nothing is read or written there. */
+
+/* Rotary positions of a step's queries and keys, with the per-head norms where
+ * a gain is given, and the append of keys and values to the pages.  The 16-bit
+ * counterpart of bq_attn_prep (butterquant/head_prep.mojo:9-92).  Token t at
+ * positions[t] of sequence seq_ids[t] (NULL: sequence t): each head of q and k
+ * is multiplied by sqrt_n / sqrt(sum of squares + n_eps) and by q_norm / k_norm
+ * [head_dim] (NULL: that tensor has no norm; norm_v: v is normed without a
+ * gain), then every pair (i, pair_stride + i), or (2 i, 2 i + 1) if pair_stride
+ * is 0, i < rope_half, turns by positions[t] * inv_freq[i] and is multiplied by
+ * mscale; the rest of the head passes.  The angle is taken in 64 bits.  Rounded
+ * once.  q goes to q_out, k and v to the token's cache row.
+ * A token with a negative position or a sequence outside [0, num_seqs) is
+ * padding: its rows are left as they were.  Where the token's page is missing,
+ * q_out is written and the cache is not.  Two tokens on one cache row leave it
+ * undefined which of the two it holds.  q_out may be q.
+ * Rows are *_stride values apart, heads contiguous.  head_dim in {64, 128, 256,
+ * 512}; pairs by halves: rope_half and pair_stride multiples of 8, rope_half <=
+ * pair_stride, pair_stride + rope_half <= head_dim; neighbouring pairs:
+ * rope_half % 4 == 0, 2 rope_half <= head_dim.  inv_freq may be NULL if
+ * rope_half is 0.  16-bit tensors 16-byte aligned, strides multiples of 8. */
+int bq_rope_append(const void* q, const void* k, const void* v, int64_t q_stride,
+                   int64_t k_stride, int64_t v_stride, const void* q_norm, const void* k_norm,
+                   int norm_v, float sqrt_n, float n_eps, const float* inv_freq, int rope_half,
+                   int pair_stride, float mscale, const int32_t* positions,
+                   const int32_t* seq_ids, const int32_t* base_rows, int num_seqs, int max_pages,
+                   int page_shift, int64_t num_slots, void* q_out, int64_t q_out_stride,
+                   void* k_cache, void* v_cache, int num_q, int num_kv, int head_dim, int dtype,
+                   int num_tokens, void* stream);
+
+/* The split count bq_paged_attention is sized for (longest sequence
+ * max_kv_len; window 0: none). */
+int bq_paged_attention_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len,
+                              int window);
+
+/* Bytes of device workspace bq_paged_attention needs for s_max splits (0 for
+ * one split). */
+size_t bq_paged_attention_workspace_size(int num_seqs, int num_q, int head_dim, int s_max);
+
+/* Attention of one new token per sequence over the pages: sequence s has
+ * kv_lens[s] cached positions, the new token's among them (clipped to its
+ * table's max_pages pages), and its num_q query heads attend to positions
+ * [max(0, len - window), len) (window 0: all) of kv head h / (num_q / num_kv):
+ * softmax of scale * q.k, or of softcap * tanh(scale * q.k / softcap) if softcap
+ * is positive.  Positions without a page take no part; what stands in rows that
+ * take no part is not looked at.  out [num_seqs, num_q * head_dim] (zeros where
+ * nothing takes part), lse [num_seqs, num_q] (may be NULL) the natural logarithm
+ * of the sum of exponentials (-inf there).  Scores, softmax and sums are 32
+ * bits; the weights are rounded to the cache's type for the product with v.
+ * kv_lens may hold more than max_kv_len, which only sizes the splits.
+ * num_q % num_kv == 0; head_dim in {64, 128, 256, 512}; s_max in [1, 256]; q,
+ * caches, out and workspace 16-byte aligned, q_stride a multiple of 8;
+ * workspace >= bq_paged_attention_workspace_size(), NULL for one split.  Calls
+ * that overlap need a workspace each. */
+int bq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                       int64_t num_slots, const int32_t* base_rows, int max_pages, int page_shift,
+                       const int32_t* kv_lens, void* out, float* lse, int num_seqs, int num_q,
+                       int num_kv, int head_dim, int window, float scale, float softcap, int dtype,
+                       int max_kv_len, int s_max, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* One array of a paged cache (host struct): num_pages << page_shift rows. */
+typedef struct bq_cache_array {
+    void* data;
+    int64_t row_bytes;
+} bq_cache_array;
+
+size_t bq_cache_reorder_workspace_size(int num_seqs);
+
+/* Sequences go on from others: sequence i continues old sequence parents[i]
+ * (outside [0, num_seqs): it is empty from here on) with room for grow[i] more
+ * positions (NULL: none).  base_rows, lens [num_seqs] and refs [num_pages] (the
+ * number of table entries that hold a page; 0 is free; other tables over the
+ * pool count too) are changed in place:
+ *   - lens[i] = the parent's length (clipped to max_pages pages);
+ *   - pages that are full are shared with the parent's other children;
+ *   - the pages of positions [lens[i], lens[i] + grow[i]) and a last page that is
+ *     not full belong to i alone: the parent's page if no one else holds it or
+ *     the others that continue on it come before i, else a fresh one, into which
+ *     the rows that it has are copied in every array;
+ *   - pages past these leave the table; pages that no one holds are free.
+ * Fresh pages are the lowest free ones, in the order (sequence, page); where the
+ * pool has none left the entry is -1.  info [4] = {fresh pages, copied pages,
+ * entries that found no page, 0}.  parents[i] = i extends, parents[i] = -1 frees.
+ * arrays (host) may be of any row size, up to 128 of them, pages whole in each.
+ * num_seqs <= 1024, num_pages << page_shift < 2^31; workspace 16-byte aligned,
+ * >= bq_cache_reorder_workspace_size().  Calls on one pool run in order. */
+int bq_cache_reorder(const bq_cache_array* arrays, int num_arrays, int32_t* base_rows,
+                     int32_t* lens, int32_t* refs, const int32_t* parents, const int32_t* grow,
+                     int num_seqs, int max_pages, int page_shift, int num_pages, int32_t* info,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+size_t bq_cache_compact_workspace_size(int num_pages);
+
+/* Packs a pool: with `live` pages held (refs not 0), the i-th free page below
+ * `live` takes the contents, count and table entries of the i-th held page from
+ * `live` on.  base_rows must be the only table over the pool.  info [4] = {live,
+ * pages moved, 0, 0}.  Limits as bq_cache_reorder. */
+int bq_cache_compact(const bq_cache_array* arrays, int num_arrays, int32_t* base_rows,
+                     int32_t* refs, int num_seqs, int max_pages, int page_shift, int num_pages,
+                     int32_t* info, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- beams ---------------------------------------------------------------------- */
+
+size_t bq_beam_select_workspace_size(int rows, int vocab);
+
+/* The n best continuations of each request: over its beams k and tokens v,
+ * scores[b, k] + logits[b * beams + k, v] - logsumexp(logits[b * beams + k, :]),
+ * in 64 bits, best first, ties to the lowest (k, v).  logits bf16, f16 or f32
+ * (BQ_DT_*), rows row_stride values apart (bq_linear's out or out_f32, for
+ * one).  A beam with finished[b, k] != 0 (finished may be NULL) is not read: it
+ * goes on as one candidate, token eos_id at its own score.  A logit or score of
+ * -inf or NaN makes no candidate, and such a logit adds nothing to the sum; a
+ * row with a logit of +inf makes none at all.
+ * out_scores [batch, n] f32, out_parents (the row b * beams + k, as
+ * bq_cache_reorder takes it when n == beams), out_tokens; where candidates run
+ * out: -inf, -1, -1.  out_finished [batch, n] (may be NULL): the parent was
+ * finished or the token is eos_id (-1: none).  Outputs may not be the inputs.
+ * beams <= 64, n <= 64, vocab <= 2^20, batch * beams <= 2^20; workspace 16-byte
+ * aligned, >= bq_beam_select_workspace_size(batch * beams, vocab). */
+int bq_beam_select(const void* logits, int64_t row_stride, int dtype, const float* scores,
+                   const uint8_t* finished, int batch, int beams, int vocab, int n, int eos_id,
+                   float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                   uint8_t* out_finished, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- on-disk weights (safetensors) -------------------------------------------- */
 
 /* safetensors dtype tags (safetensors/parser.mojo:19-54) */

@@ -24,7 +24,7 @@ class BqError(RuntimeError):
         self.code = code
 
 
-_vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_vp, _i, _f, _sz, _l = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_int64
 
 # symbol -> argtypes (restype int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -77,11 +77,28 @@ SIGNATURES = {
                                    _i, _vp],
     "bq_ffn_gate_up": [_vp] * 8 + [_i] * 5 + [_vp] * 6 + [_i] + [_vp] * 3,
     "bq_ffn_down": [_vp] * 8 + [_i] * 6 + [_vp] * 4 + [_i, _vp, _vp, _sz, _vp],
+    "bq_rope_append": [_vp] * 3 + [_l] * 3 + [_vp, _vp, _i, _f, _f, _vp, _i, _i, _f, _vp, _vp, _vp,
+                       _i, _i, _i, _l, _vp, _l, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "bq_paged_attention_splits": [_i] * 6,
+    "bq_paged_attention_workspace_size": [_i] * 4,
+    "bq_paged_attention": [_vp, _l, _vp, _vp, _l, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+                           _f, _f, _i, _i, _i, _vp, _sz, _vp],
+    "bq_cache_reorder_workspace_size": [_i],
+    "bq_cache_reorder": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp],
+    "bq_cache_compact_workspace_size": [_i],
+    "bq_cache_compact": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp],
+    "bq_beam_select_workspace_size": [_i, _i],
+    "bq_beam_select": [_vp, _l, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz,
+                       _vp],
 }
 _RESTYPES = {"bq_last_error": C.c_char_p, "bq_version": C.c_char_p,
              "bq_moe_phase2_workspace_size": C.c_size_t,
              "bq_flash_sample_workspace_size": C.c_size_t, "bq_st_close": None,
-             "bq_attention_workspace_size": C.c_size_t}
+             "bq_attention_workspace_size": C.c_size_t,
+             "bq_paged_attention_workspace_size": C.c_size_t,
+             "bq_cache_reorder_workspace_size": C.c_size_t,
+             "bq_cache_compact_workspace_size": C.c_size_t,
+             "bq_beam_select_workspace_size": C.c_size_t}
 
 
 def _load():
@@ -761,6 +778,287 @@ def attention(q_i8, qi_bias, f_q, k_cache, k_scale, v_cache, v_scale, runs, base
                                     _stream())
     _check(rc)
     return out, s_max
+
+
+# --------------------------------------------------------------------------
+# paged 16-bit cache and beams
+# --------------------------------------------------------------------------
+_DTYPES = {torch.float16: 5, torch.float32: 9, torch.bfloat16: 6}  # BQ_DT_*
+
+
+def _half(*tensors):
+    """The BQ_DT_* of 16-bit device tensors of one type."""
+    dt = tensors[0].dtype
+    if dt not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"expected bfloat16 or float16, got {dt}")
+    for t in tensors:
+        if t is not None and t.dtype != dt:
+            raise TypeError(f"expected {dt} throughout, got {t.dtype}")
+    return _DTYPES[dt]
+
+
+def _here(*tensors):
+    """Every tensor on the current device, whose current stream the call takes."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise ValueError(f"libbq launches on the current device cuda:{dev}; got a tensor on "
+                             f"{t.device}")
+
+
+def _rows(t: torch.Tensor, width: int):
+    """The row stride of a [rows, width] tensor whose rows are contiguous."""
+    if t.dim() != 2 or t.shape[1] != width:
+        raise ValueError(f"expected [rows, {width}], got {tuple(t.shape)}")
+    if width > 1 and t.stride(1) != 1:
+        raise ValueError("libbq takes rows of contiguous values")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _table(base_rows: torch.Tensor):
+    _dev(base_rows, torch.int32)
+    if base_rows.dim() != 2:
+        raise ValueError("base_rows: int32 [sequences, pages]")
+    return base_rows.shape
+
+
+def _flat(t: torch.Tensor, dtype, n: int, name: str):
+    """A contiguous [n] tensor (of any shape with n values)."""
+    _dev(t, dtype)
+    if t.numel() != n:
+        raise ValueError(f"{name}: expected {n} values, got {tuple(t.shape)}")
+    return t
+
+
+def rope_frequencies(rope_half: int, base: float = 10000.0, factor: float = 1.0,
+                     original_len: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                     device="cuda"):
+    """-> (inv_freq f32 [rope_half], mscale) for rope_append.  factor 1: base **
+    (-i / rope_half), mscale 1.  factor > 1 stretches a model made for
+    original_len positions to factor times as many: original_len 0 divides every
+    frequency by it (linear); otherwise (YaRN, Peng et al. 2023) pairs that turn
+    more than beta_fast times within original_len keep their frequency, those
+    that turn less than beta_slow times are divided, with a ramp between, and
+    mscale = 0.1 ln(factor) + 1."""
+    import math
+    if rope_half <= 0 or not base > 1.0 or not factor >= 1.0:
+        raise ValueError("rope_frequencies: need rope_half > 0, base > 1, factor >= 1")
+    i = torch.arange(rope_half, dtype=torch.float64)
+    f = base ** (-i / rope_half)
+    mscale = 1.0
+    if factor > 1.0 and original_len > 0:
+        if not beta_fast > beta_slow > 0.0:
+            raise ValueError("rope_frequencies: need beta_fast > beta_slow > 0")
+        pair = lambda turns: rope_half * math.log(original_len / (turns * 2 * math.pi)) / math.log(base)
+        lo, hi = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rope_half - 1)
+        ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        f = f * (1.0 - ramp) + f / factor * ramp
+        mscale = 0.1 * math.log(factor) + 1.0
+    elif factor > 1.0:
+        f = f / factor
+    return f.to(torch.float32).to(device), mscale
+
+
+def rope_append(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, num_q: int, num_kv: int,
+                head_dim: int, page_shift: int, pair_stride: int | None = None,
+                mscale: float = 1.0, seq_ids=None, q_norm=None, k_norm=None, norm_v: bool = False,
+                sqrt_n: float | None = None, n_eps: float | None = None, out=None):
+    """bq_rope_append: norms, rotary positions and the append to the pages ->
+    q [T, num_q*hd] (out may be q itself); k and v go into k_cache / v_cache
+    [slots, num_kv*hd].  q, k, v are bf16 or f16 [T, heads*hd], their rows may be
+    parts of a wider buffer.  inv_freq f32 [rope_half] or None (no rotation);
+    pair_stride None: rope_half (pairs by halves), 0: neighbours."""
+    dt = _half(q, k, v, k_cache, v_cache, q_norm, k_norm, out)
+    _here(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, seq_ids, q_norm, k_norm, out)
+    T, kw = q.shape[0], num_kv * head_dim
+    qs, ks, vs = _rows(q, num_q * head_dim), _rows(k, kw), _rows(v, kw)
+    if k.shape[0] != T or v.shape[0] != T:
+        raise ValueError(f"rope_append: {T} rows of q, {k.shape[0]} of k, {v.shape[0]} of v")
+    for c in (k_cache, v_cache):
+        _dev(c)
+        if c.dim() != 2 or c.shape[1] != kw or c.shape[0] != k_cache.shape[0]:
+            raise ValueError(f"caches: expected [slots, {kw}] twice, got {tuple(k_cache.shape)} and "
+                             f"{tuple(v_cache.shape)}")
+    _flat(positions, torch.int32, T, "positions")
+    if seq_ids is not None:
+        _flat(seq_ids, torch.int32, T, "seq_ids")
+    for g in (q_norm, k_norm):
+        if g is not None:
+            _flat(g, None, head_dim, "gain")
+    half = 0 if inv_freq is None else _dev(inv_freq, torch.float32).numel()
+    n, width = _table(base_rows)
+    if sqrt_n is None or n_eps is None:
+        sqrt_n, n_eps = head_dim ** 0.5, head_dim * 1e-6
+    if out is None:
+        out = torch.empty((T, num_q * head_dim), dtype=q.dtype, device=q.device)
+    os_ = _rows(out, num_q * head_dim)
+    if out.shape[0] != T:
+        raise ValueError(f"out: expected {T} rows, got {out.shape[0]}")
+    _check(_lib.bq_rope_append(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, _p(q_norm), _p(k_norm), int(norm_v),
+        sqrt_n, n_eps, _p(inv_freq), half, half if pair_stride is None else pair_stride, mscale,
+        positions.data_ptr(), _p(seq_ids), base_rows.data_ptr(), n, width, page_shift,
+        k_cache.shape[0], out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), num_q,
+        num_kv, head_dim, dt, T, _stream()))
+    return out
+
+
+def paged_attention_splits(num_seqs: int, num_q: int, num_kv: int, head_dim: int,
+                           max_kv_len: int, window: int = 0) -> int:
+    return int(_lib.bq_paged_attention_splits(num_seqs, num_q, num_kv, head_dim, max_kv_len,
+                                              window))
+
+
+def paged_attention_workspace(num_seqs: int, num_q: int, head_dim: int, s_max: int,
+                              device="cuda"):
+    n = int(_lib.bq_paged_attention_workspace_size(num_seqs, num_q, head_dim, s_max))
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv: int,
+                    head_dim: int, page_shift: int, window: int = 0, scale: float | None = None,
+                    softcap: float = 0.0, max_kv_len: int | None = None, s_max: int | None = None,
+                    workspace=None, out=None, lse=None):
+    """bq_paged_attention: one new token per sequence over the pages -> [S,
+    num_q*hd] of q's type (bf16 or f16).  kv_lens int32 [S], the new token's
+    position among them.  max_kv_len sizes the splits (None: the table's);
+    scale None: head_dim ** -0.5; lse: f32 [S, num_q] to fill."""
+    dt = _half(q, k_cache, v_cache, out)
+    _here(q, k_cache, v_cache, base_rows, kv_lens, workspace, out, lse)
+    S, kw = q.shape[0], num_kv * head_dim
+    qs = _rows(q, num_q * head_dim)
+    for c in (k_cache, v_cache):
+        _dev(c)
+        if c.dim() != 2 or c.shape[1] != kw or c.shape[0] != k_cache.shape[0]:
+            raise ValueError(f"caches: expected [slots, {kw}] twice, got {tuple(k_cache.shape)} and "
+                             f"{tuple(v_cache.shape)}")
+    n, width = _table(base_rows)
+    if n < S:
+        raise ValueError(f"base_rows: {n} rows for {S} sequences")
+    _flat(kv_lens, torch.int32, S, "kv_lens")
+    if max_kv_len is None:
+        max_kv_len = min(width << page_shift, 2**31 - 1)
+    if s_max is None:
+        s_max = paged_attention_splits(S, num_q, num_kv, head_dim, max_kv_len, window)
+    if workspace is None:
+        workspace = paged_attention_workspace(S, num_q, head_dim, s_max, q.device)
+    if out is None:
+        out = torch.empty((S, num_q * head_dim), dtype=q.dtype, device=q.device)
+    _flat(out, None, S * num_q * head_dim, "out")
+    if lse is not None:
+        _flat(lse, torch.float32, S * num_q, "lse")
+    _check(_lib.bq_paged_attention(
+        q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
+        base_rows.data_ptr(), width, page_shift, kv_lens.data_ptr(), out.data_ptr(), _p(lse), S,
+        num_q, num_kv, head_dim, window, head_dim ** -0.5 if scale is None else scale, softcap, dt,
+        max_kv_len, s_max, _p(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()))
+    return out
+
+
+class _CacheArray(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("row_bytes", C.c_int64)]
+
+
+def _cache_arrays(arrays, slots: int):
+    """The host table of a cache's arrays ([slots, ...] each) for one call."""
+    table = (_CacheArray * max(len(arrays), 1))()
+    for i, a in enumerate(arrays):
+        _dev(a)
+        if a.dim() < 1 or a.shape[0] != slots or a.numel() == 0:
+            raise ValueError(f"array {i}: expected {slots} rows, got {tuple(a.shape)}")
+        table[i].data = a.data_ptr()
+        table[i].row_bytes = a.numel() // slots * a.element_size()
+    return table
+
+
+def cache_reorder(arrays, base_rows, lens, refs, parents, page_shift: int, grow=None,
+                  workspace=None, info=None):
+    """bq_cache_reorder: sequence i goes on as old sequence parents[i] (-1: empty)
+    with room for grow[i] more positions; base_rows [N, pages], lens [N], refs
+    [pool] change in place, written pages are copied in every array ([pool <<
+    page_shift, ...]) -> info int32 [4] (fresh, copied, missing, 0)."""
+    _here(base_rows, lens, refs, parents, grow, workspace, info, *arrays)
+    n, width = _table(base_rows)
+    _flat(lens, torch.int32, n, "lens")
+    _flat(parents, torch.int32, n, "parents")
+    if grow is not None:
+        _flat(grow, torch.int32, n, "grow")
+    pool = _dev(refs, torch.int32).numel()
+    table = _cache_arrays(arrays, pool << page_shift)
+    if workspace is None:
+        workspace = torch.empty(int(_lib.bq_cache_reorder_workspace_size(n)), dtype=torch.uint8,
+                                device=base_rows.device)
+    if info is None:
+        info = torch.empty(4, dtype=torch.int32, device=base_rows.device)
+    _flat(info, torch.int32, 4, "info")
+    _check(_lib.bq_cache_reorder(table, len(arrays), base_rows.data_ptr(), lens.data_ptr(),
+                                 refs.data_ptr(), parents.data_ptr(), _p(grow), n, width,
+                                 page_shift, pool, info.data_ptr(), workspace.data_ptr(),
+                                 workspace.numel() * workspace.element_size(), _stream()))
+    return info
+
+
+def cache_compact(arrays, base_rows, refs, page_shift: int, workspace=None, info=None):
+    """bq_cache_compact: the held pages move below their number; base_rows, refs
+    and every array change in place -> info int32 [4] (held, moved, 0, 0)."""
+    _here(base_rows, refs, workspace, info, *arrays)
+    n, width = _table(base_rows)
+    pool = _dev(refs, torch.int32).numel()
+    table = _cache_arrays(arrays, pool << page_shift)
+    if workspace is None:
+        workspace = torch.empty(int(_lib.bq_cache_compact_workspace_size(pool)),
+                                dtype=torch.uint8, device=base_rows.device)
+    if info is None:
+        info = torch.empty(4, dtype=torch.int32, device=base_rows.device)
+    _flat(info, torch.int32, 4, "info")
+    _check(_lib.bq_cache_compact(table, len(arrays), base_rows.data_ptr(), refs.data_ptr(), n,
+                                 width, page_shift, pool, info.data_ptr(), workspace.data_ptr(),
+                                 workspace.numel() * workspace.element_size(), _stream()))
+    return info
+
+
+def beam_select(logits, scores, n: int | None = None, finished=None, eos_id: int = -1,
+                workspace=None, out=None):
+    """bq_beam_select: the n best of beams x vocab for each request -> (scores
+    f32 [B, n], parents int32 [B, n] as rows of logits, tokens int32 [B, n]), and
+    finished uint8 [B, n] where finished [B, K] (uint8 or bool) is given.
+    logits bf16, f16 or f32 [B*K, vocab], scores f32 [B, K]; n None: K."""
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"expected bfloat16, float16 or float32, got {logits.dtype}")
+    _dev(scores, torch.float32)
+    if scores.dim() != 2 or logits.dim() != 2:
+        raise ValueError("scores: [requests, beams], logits: [requests * beams, vocab]")
+    _here(logits, scores, finished, workspace)
+    b, k = scores.shape
+    rows, vocab = logits.shape
+    if rows != b * k:
+        raise ValueError(f"logits: expected {b * k} rows, got {rows}")
+    stride = _rows(logits, vocab)
+    if n is None:
+        n = k
+    if finished is not None:
+        _flat(finished, torch.bool if finished.dtype == torch.bool else torch.uint8, b * k,
+              "finished")
+    d = logits.device
+    if workspace is None:
+        workspace = torch.empty(int(_lib.bq_beam_select_workspace_size(rows, vocab)),
+                                dtype=torch.uint8, device=d)
+    if out is None:
+        out = (torch.empty((b, n), dtype=torch.float32, device=d),
+               torch.empty((b, n), dtype=torch.int32, device=d),
+               torch.empty((b, n), dtype=torch.int32, device=d))
+        if finished is not None:
+            out += (torch.empty((b, n), dtype=torch.uint8, device=d),)
+    for t, dt in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8)):
+        _flat(t, dt, b * n, "out")
+    _here(*out)
+    _check(_lib.bq_beam_select(logits.data_ptr(), stride, _DTYPES[logits.dtype],
+                               scores.data_ptr(), _p(finished), b, k, vocab, n, eos_id,
+                               out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+                               out[3].data_ptr() if len(out) > 3 else None, workspace.data_ptr(),
+                               workspace.numel() * workspace.element_size(), _stream()))
+    return out
 
 
 # --------------------------------------------------------------------------

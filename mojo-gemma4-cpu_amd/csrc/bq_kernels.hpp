@@ -238,4 +238,72 @@ hipError_t launch_attn_prep(const PrepArgs& a, int head_dim, hipStream_t st);
 hipError_t launch_flash_attn(const AttnArgs& a, int head_dim, hipStream_t st);
 int attn_splits(int seq_len, int num_kv, int max_kv_len);
 
+// the paged 16-bit cache and beams (bq_rope.hip, bq_paged_attn.hip, bq_cache.hip,
+// bq_beam.hip); the page table is described in bq_pages.hpp
+struct RopeArgs {
+  const uint16_t *q, *k, *v;              // [tokens, heads * head_dim], rows *_stride values apart
+  int64_t q_stride, k_stride, v_stride;
+  const uint16_t *q_norm, *k_norm;        // [head_dim] or null: no norm
+  const float* inv_freq;                  // [rope_half]
+  const int32_t *positions, *seq_ids;     // [tokens]; seq_ids null: token t is sequence t's
+  const int32_t* base_rows;               // [num_seqs, max_pages]
+  uint16_t *q_out, *k_cache, *v_cache;
+  int64_t q_out_stride, num_slots;
+  int num_tokens, num_seqs, max_pages, page_shift, num_q, num_kv, rope_half, pair_stride, norm_v;
+  float mscale, sqrt_n, n_eps;
+};
+struct PagedAttnArgs {
+  const uint16_t* q;                      // [num_seqs, num_q * head_dim], rows q_stride apart
+  int64_t q_stride, num_slots;
+  const uint16_t *k_cache, *v_cache;      // [num_slots, num_kv * head_dim]
+  const int32_t *base_rows, *kv_lens;     // [num_seqs, max_pages], [num_seqs]
+  uint16_t* out;                          // [num_seqs, num_q * head_dim]
+  float* lse;                             // [num_seqs, num_q] or null
+  float *ws_acc, *ws_ml;                  // [num_seqs, num_q, s_max] x head_dim and x 2
+  int num_seqs, num_q, num_kv, gqa, head_groups, max_pages, page_shift, window, s_max;
+  int chunk_tiles;                        // the launcher's: tiles per split
+  float scale2, softcap2, inv_cap;        // score factors (see bq_paged_attn.hip)
+};
+constexpr int kMaxCacheSeqs = 1024, kMaxCacheArrays = 128;
+struct CacheArrays {                      // what the pages hold: [num_pages << page_shift] rows each
+  int n;
+  void* data[kMaxCacheArrays];
+  int64_t row_bytes[kMaxCacheArrays];
+};
+struct ReorderArgs {
+  int32_t *base_rows, *lens, *refs;       // [num_seqs, max_pages], [num_seqs], [num_pages]
+  const int32_t *parents, *grow;          // [num_seqs]; grow may be null
+  int32_t* info;                          // [4]
+  void* workspace;
+  int num_seqs, max_pages, page_shift, num_pages;
+};
+struct CompactArgs {
+  int32_t *base_rows, *refs, *info;
+  void* workspace;
+  int num_seqs, max_pages, page_shift, num_pages;
+};
+constexpr int kMaxBeams = 64, kMaxPicks = 64;
+struct BeamArgs {
+  const void* logits;                     // [batch * beams, vocab], rows row_stride apart
+  int64_t row_stride;
+  const float* scores;                    // [batch, beams]
+  const uint8_t* finished;                // [batch, beams] or null
+  float* out_scores;                      // [batch, n]
+  int32_t *out_parents, *out_tokens;
+  uint8_t* out_finished;                  // or null
+  void* workspace;
+  int batch, beams, vocab, n, eos_id, parts;
+};
+hipError_t launch_rope_append(const RopeArgs& a, int head_dim, bool f16, hipStream_t st);
+int paged_attn_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len, int window);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, int max_len, bool f16,
+                             hipStream_t st);
+size_t reorder_workspace(int num_seqs);
+size_t compact_workspace(int num_pages);
+hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays, hipStream_t st);
+hipError_t launch_cache_compact(const CompactArgs& a, const CacheArrays& arrays, hipStream_t st);
+int beam_parts(int vocab);
+size_t beam_workspace(int64_t rows, int vocab);
+hipError_t launch_beam_select(const BeamArgs& a, int dtype_bytes, bool f16, hipStream_t st);
+
 }  // namespace bq

@@ -1,0 +1,367 @@
+// Attention of one new token per sequence over the paged 16-bit cache.
+//
+// Reference: kernels/attention_ops.mojo:45-51 (PagedKV), :166-182 (online
+// softmax of a tile), kernels/logsum_merge.mojo:29-122 (merge of the splits).
+//
+// Sequence s has one query row per head, at position len - 1, and attends to the
+// cached positions [max(0, len - window), len):
+//   x_p = cap tanh(scale q.k_p / cap),  o = sum_p e^(x_p) v_p / sum_p e^(x_p).
+//
+// Bound: the cache rows, 2 len num_kv head_dim 16-bit values per sequence, are
+// read once; the arithmetic is 2 num_q / num_kv operations a byte.
+//
+// A wave walks tiles of TP positions for up to 16 query heads of one kv head.
+// Scores: A = 16 cache rows, B = the 16 query heads (those past the group are
+// zero), so a lane ends with 4 positions of one head per 16 rows.  That is the
+// layout in which the next product takes its B operand when a tile's positions
+// are read as its k index in the order (group of 16, quad, row): the weights go
+// from one product to the next in their lane.  The values are the other operand,
+// transposed, as O^T = V^T P^T: a lane reads 8 columns of its positions (16 lanes:
+// 256 contiguous bytes of a row) and pairs positions with one byte permute per
+// two values.  No LDS and no cross-lane traffic but the maxima.
+// Weights are rounded to the cache's type for that product (each by 2^-9 or 2^-12
+// of itself; their sum is taken from the unrounded ones in 32 bits); scores,
+// maxima, sums and outputs are 32 bits until the one rounding at the end.
+//
+// The waves of a workgroup take every NW-th tile of a range and join in LDS;
+// ranges of one sequence are joined by k_paged_merge in their order.
+#include <algorithm>
+
+#include "bq_half.hpp"
+#include "bq_kernels.hpp"
+#include "bq_pages.hpp"
+
+namespace bq {
+
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// over the four lanes l % 16 + {0, 16, 32, 48}
+__device__ inline float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float quad_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// a sequence's positions and the tiles of them that split `split` takes
+struct Range {
+  int len, start;  // positions [start, len)
+  int t0, t1;      // tiles of TP positions, absolute
+  int splits;      // of this sequence
+};
+
+__device__ inline Range attn_range(const PagedAttnArgs& a, int seq, int split, int tp) {
+  Range r;
+  const int64_t room = (int64_t)a.max_pages << a.page_shift;
+  int64_t len = a.kv_lens[seq];
+  len = len < room ? len : room;
+  r.len = (int)(len > 0 ? len : 0);
+  r.start = a.window > 0 && r.len > a.window ? r.len - a.window : 0;
+  const int first = r.start / tp, end = (r.len + tp - 1) / tp;
+  int n = (end - first + a.chunk_tiles - 1) / a.chunk_tiles;
+  r.splits = n < a.s_max ? n : a.s_max;
+  r.t0 = first + split * a.chunk_tiles;
+  // the last split takes what a sequence longer than the plan's has left
+  r.t1 = split == r.splits - 1 ? end : r.t0 + a.chunk_tiles;
+  if (split >= r.splits) r.t1 = r.t0;
+  return r;
+}
+
+// HD = 512 takes 16 positions a tile: K, V, the queries and the accumulators of
+// 32 would pass the 512 registers of a lane.
+template <int HD>
+constexpr int tile_positions() {
+  return HD == 512 ? 16 : 32;
+}
+
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
+  constexpr int TP = tile_positions<HD>();
+  constexpr int KS = HD / 32;            // steps of the score product
+  constexpr int MT = TP / 16;            // groups of 16 positions
+  constexpr int CPL = HD == 64 ? 4 : 8;  // value columns per lane and group
+  constexpr int CG = HD / (16 * CPL);    // column groups
+  constexpr int VW = CPL / 2;            // words of a value load
+  constexpr int NP = TP / 4;             // positions per lane of the value product
+  constexpr int LD = HD + 8;             // LDS row: 16 heads 32 bytes apart in the banks
+
+  extern __shared__ float smem[];  // acc [NW][G][LD], then m, l [NW][16] each
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  const int n16 = lane & 15, quad = lane >> 4;
+
+  int b = blockIdx.x;
+  const int split = b % a.s_max;
+  b /= a.s_max;
+  const int hg = b % a.head_groups;
+  b /= a.head_groups;
+  const int kvh = b % a.num_kv, seq = b / a.num_kv;
+  const int G = min(16, a.gqa - hg * 16);
+  const int head0 = kvh * a.gqa + hg * 16;
+
+  const Range rg = attn_range(a, seq, split, TP);
+  if (split > 0 && split >= rg.splits) return;  // split 0 also writes empty rows
+
+  v4u qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = v4u{0, 0, 0, 0};
+  if (n16 < G) {
+    const uint16_t* q = a.q + (int64_t)seq * a.q_stride + (int64_t)(head0 + n16) * HD + quad * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const v4u*>(q + ks * 32);
+  }
+
+  const int32_t* rows = a.base_rows + (int64_t)seq * a.max_pages;
+  const int64_t stride = (int64_t)a.num_kv * HD;
+  const uint16_t* kc = a.k_cache + (int64_t)kvh * HD + quad * 8;
+  const uint16_t* vc = a.v_cache + (int64_t)kvh * HD + n16 * CPL;
+
+  v4f32 o[CG][CPL];
+#pragma unroll
+  for (int i = 0; i < CG; ++i)
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) o[i][c] = v4f32{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  for (int t = rg.t0 + wave; t < rg.t1; t += NW) {
+    const int p0 = t * TP;
+    // slots of the tile's rows, and which of its positions take part
+    uint32_t ok;
+    int64_t kslot[MT], vslot[NP];
+    {
+      const int p = p0 + (lane & (TP - 1));
+      const bool in = p >= rg.start && p < rg.len;
+      const int64_t s = in ? page_slot(rows, a.max_pages, a.page_shift, a.num_slots, p) : -1;
+      ok = (uint32_t)(__ballot(s >= 0)) & (uint32_t)((1ull << TP) - 1);
+      const int sl = s < 0 ? 0 : (int)s;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) kslot[i] = __shfl(sl, i * 16 + n16);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) vslot[j] = __shfl(sl, (j >> 2) * 16 + quad * 4 + (j & 3));
+    }
+    v4u kf[MT][KS];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const uint16_t* p = kc + kslot[i] * stride;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[i][ks] = *reinterpret_cast<const v4u*>(p + ks * 32);
+    }
+    uint32_t vf[CG][NP][VW];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const uint16_t* p = vc + vslot[j] * stride;
+#pragma unroll
+      for (int i = 0; i < CG; ++i) {
+        if constexpr (VW == 4) {
+          const v4u w = *reinterpret_cast<const v4u*>(p + i * 128);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) vf[i][j][x] = w[x];
+        } else {
+          const v2u w = *reinterpret_cast<const v2u*>(p);
+          vf[i][j][0] = w[0];
+          vf[i][j][1] = w[1];
+        }
+      }
+    }
+    // scores in powers of two, -inf where a position takes no part
+    float x[NP];
+    float mt = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      v4f32 s = {0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = T::mfma32(kf[i][ks], qf[ks], s);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float y = s[r] * a.scale2;
+        if (a.softcap2 > 0.0f) {  // cap tanh(y / cap), tanh z = 1 - 2 / (e^2z + 1)
+          const float e = exp2_(y * a.inv_cap);
+          y = a.softcap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f));
+        }
+        y = (ok >> (i * 16 + quad * 4 + r)) & 1 ? y : -INFINITY;
+        x[i * 4 + r] = y;
+        mt = fmaxf(mt, y);
+      }
+    }
+    const float mn = fmaxf(m, quad_max(mt));
+    const float ms = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = exp2_(m - ms), mw = ms - T::kWeightBits;
+    m = mn;
+    uint32_t pf[NP / 2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NP; j += 2) {
+      const float p0_ = exp2_(x[j] - mw), p1_ = exp2_(x[j + 1] - mw);
+      sum += p0_ + p1_;
+      pf[j / 2] = T::pack(p0_, p1_);
+    }
+    l = fmaf(l, alpha, sum);
+    if (ok != (uint32_t)((1ull << TP) - 1)) {  // what stands in other rows may be anything
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+        if (!((ok >> ((j >> 2) * 16 + quad * 4 + (j & 3))) & 1))
+#pragma unroll
+          for (int i = 0; i < CG; ++i)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vf[i][j][w] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < CG; ++i)
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) {
+        const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t vt[NP / 2];
+#pragma unroll
+        for (int j = 0; j < NP / 2; ++j)
+          vt[j] = __builtin_amdgcn_perm(vf[i][2 * j + 1][c / 2], vf[i][2 * j][c / 2], sel);
+        v4f32 acc = o[i][c] * alpha;
+        if constexpr (NP == 8)
+          acc = T::mfma32(v4u{vt[0], vt[1], vt[2], vt[3]}, v4u{pf[0], pf[1], pf[2], pf[3]}, acc);
+        else
+          acc = T::mfma16(v2u{vt[0], vt[1]}, v2u{pf[0], pf[1]}, acc);
+        o[i][c] = acc;
+      }
+  }
+  l = quad_sum(l);
+
+  // the waves' parts, joined in LDS: o[i][c][r] is column i 16 CPL + (4 quad + r) CPL + c
+  float* sm = smem + (size_t)NW * G * LD;
+  if (n16 < G) {
+    float* d = smem + ((size_t)wave * G + n16) * LD;
+#pragma unroll
+    for (int i = 0; i < CG; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < CPL; c += 4)
+          *reinterpret_cast<v4f32*>(d + i * 16 * CPL + (quad * 4 + r) * CPL + c) =
+              v4f32{o[i][c][r], o[i][c + 1][r], o[i][c + 2][r], o[i][c + 3][r]};
+    if (quad == 0) {
+      sm[wave * 16 + n16] = m;
+      sm[NW * 16 + wave * 16 + n16] = l;
+    }
+  }
+  __syncthreads();
+  const bool whole = rg.splits <= 1;
+  for (int e = threadIdx.x; e < G * (HD / 4); e += NW * 64) {
+    const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w * 16 + h]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    v4f32 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = exp2_(sm[w * 16 + h] - Ms);
+      L = fmaf(f, sm[NW * 16 + w * 16 + h], L);
+      const v4f32 v = *reinterpret_cast<const v4f32*>(smem + ((size_t)w * G + h) * LD + col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+    }
+    const int64_t row = (int64_t)seq * a.num_q + head0 + h;
+    if (whole) {
+      const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // a NaN sum stays
+      v2u w = {T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+      *reinterpret_cast<v2u*>(a.out + row * HD + col) = w;
+      if (a.lse && col == 0) a.lse[row] = L != 0.0f ? (M + __builtin_amdgcn_logf(L) - T::kWeightBits) * kLn2 : -INFINITY;
+    } else {
+      *reinterpret_cast<v4f32*>(a.ws_acc + (row * a.s_max + split) * HD + col) = acc;
+      if (col == 0) {
+        float* ml = a.ws_ml + (row * a.s_max + split) * 2;
+        ml[0] = M;
+        ml[1] = L;
+      }
+    }
+  }
+}
+
+// Joins a row's splits in their order: HD / 4 lanes a row, four columns each.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a) {
+  constexpr int TPR = HD / 4, RPB = 256 / TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (row >= (int64_t)a.num_seqs * a.num_q) return;
+  const int seq = (int)(row / a.num_q), col = (threadIdx.x % TPR) * 4;
+  const int S = attn_range(a, seq, 0, tile_positions<HD>()).splits;
+  if (S <= 1) return;
+  const float* ml = a.ws_ml + row * a.s_max * 2;
+  const float* acc = a.ws_acc + row * a.s_max * HD + col;
+  float M = -INFINITY;
+  for (int s = 0; s < S; ++s) M = fmaxf(M, ml[2 * s]);
+  const float Ms = M == -INFINITY ? 0.0f : M;
+  float L = 0.0f;
+  v4f32 r = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < S; ++s) {
+    const float f = exp2_(ml[2 * s] - Ms);
+    L = fmaf(f, ml[2 * s + 1], L);
+    const v4f32 v = *reinterpret_cast<const v4f32*>(acc + (int64_t)s * HD);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fmaf(f, v[i], r[i]);
+  }
+  const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+  v2u w = {T::pack(r[0] * inv, r[1] * inv), T::pack(r[2] * inv, r[3] * inv)};
+  *reinterpret_cast<v2u*>(a.out + row * HD + col) = w;
+  if (a.lse && col == 0) a.lse[row] = L != 0.0f ? (M + __builtin_amdgcn_logf(L) - T::kWeightBits) * kLn2 : -INFINITY;
+}
+
+template <typename T, int HD>
+hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
+  constexpr int NW = 4, TP = tile_positions<HD>();
+  // a window that does not start on a tile reaches into one more
+  const int tiles = (max_len + TP - 1) / TP + (a.window > 0 ? 1 : 0);
+  a.chunk_tiles = std::max(1, (tiles + a.s_max - 1) / a.s_max);
+  const int G = std::min(16, a.gqa);
+  const int64_t blocks = (int64_t)a.num_seqs * a.num_kv * a.head_groups * a.s_max;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  const size_t lds = ((size_t)NW * G * (HD + 8) + 2 * NW * 16) * sizeof(float);
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_attn<T, HD, NW>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  k_paged_attn<T, HD, NW><<<(int)blocks, NW * 64, lds, st>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.s_max == 1) return e;
+  const int rpb = 256 / (HD / 4);
+  const int64_t rows = (int64_t)a.num_seqs * a.num_q;
+  k_paged_merge<T, HD><<<(int)((rows + rpb - 1) / rpb), 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_hd(const PagedAttnArgs& a, int hd, int max_len, hipStream_t st) {
+  switch (hd) {
+    case 64: return launch<T, 64>(a, max_len, st);
+    case 128: return launch<T, 128>(a, max_len, st);
+    case 256: return launch<T, 256>(a, max_len, st);
+    default: return launch<T, 512>(a, max_len, st);
+  }
+}
+
+}  // namespace
+
+// Workgroups of 4 waves, a tile a wave at a time: enough splits for `target`
+// workgroups, none of fewer than four tiles.
+int paged_attn_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len, int window) {
+  const int tp = head_dim == 512 ? 16 : 32;
+  int64_t len = window > 0 ? std::min(max_kv_len, window) : max_kv_len;
+  const int64_t tiles = (len + tp - 1) / tp + (window > 0 ? 1 : 0);
+  const int64_t groups = (int64_t)num_seqs * num_kv * ((num_q / num_kv + 15) / 16);
+  const int64_t target = 512;
+  const int64_t s = std::min((target + groups - 1) / groups, (tiles + 3) / 4);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, 256));
+}
+
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, int max_len, bool f16,
+                             hipStream_t st) {
+  return f16 ? launch_hd<F16>(a, head_dim, max_len, st) : launch_hd<Bf16>(a, head_dim, max_len, st);
+}
+
+}  // namespace bq

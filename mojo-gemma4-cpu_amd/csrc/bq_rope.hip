@@ -1,0 +1,180 @@
+// Rotary positions of a step's queries and keys, with the per-head RMS norms
+// where the model has them, and the writing of keys and values into the pages
+// of the 16-bit cache.
+//
+// Reference: butterquant/head_prep.mojo:9-36 (the norm and rotation of a head,
+// there ahead of the int8 rotation), kernels/attention_ops.mojo:45-51 (PagedKV).
+//
+// Per token at position p and pair i < rope_half: angle = p * inv_freq[i],
+//   (a, b) -> mscale * (a cos - b sin, b cos + a sin)
+// on the pairs (i, pair_stride + i), or (2i, 2i + 1) where pair_stride is 0;
+// the rest of a head passes.  The angle is one product in 64 bits, as turns,
+// and its whole turns are taken off there: at position 2^20 an angle in 32 bits
+// is off by up to 2^-5 rad.  What is left, at most half a turn, goes to the
+// sine and cosine instructions in 32 bits (2^-25 turns).
+#include "bq_half.hpp"
+#include "bq_kernels.hpp"
+#include "bq_pages.hpp"
+
+namespace bq {
+
+namespace {
+
+struct RopeHead {
+  const uint16_t* src;
+  uint16_t* dst;        // null: not written
+  const uint16_t* gain;  // null: none
+  bool norm, turn, on;
+};
+
+// A wave takes 64 / LPH heads of one token at a time, head_dim / 8 = LPH lanes
+// a head and 8 values a lane, IT times over, so that the sines of a lane's
+// pairs serve IT heads.
+template <typename T, int LPH, int IT>
+__global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
+  constexpr int HPW = 64 / LPH, HD = LPH * 8;
+  const int heads = a.num_q + 2 * a.num_kv;
+  const int groups = (heads + HPW * IT - 1) / (HPW * IT);
+  const int64_t work = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t tok64 = work / groups;
+  if (tok64 >= a.num_tokens) return;
+  const int tok = __builtin_amdgcn_readfirstlane((int)tok64);
+  const int group = __builtin_amdgcn_readfirstlane((int)(work - tok64 * groups));
+  const int lane = lane_id(), c = lane % LPH, sub = lane / LPH;
+
+  const int pos = a.positions[tok];
+  const int seq = a.seq_ids ? a.seq_ids[tok] : tok;
+  if (pos < 0 || seq < 0 || seq >= a.num_seqs) return;  // padding
+  const int64_t slot = page_slot(a.base_rows + (int64_t)seq * a.max_pages, a.max_pages,
+                                 a.page_shift, a.num_slots, pos);
+
+  // this lane's pairs: values 8c .. 8c + 7 of a head, their partners in chunk pc
+  int pc = c, i0 = 0;
+  float sign = 0.0f;  // partner's sine term: -1 first of a pair, +1 second, 0 passes
+  if (a.pair_stride == 0) {
+    i0 = 4 * c;
+    sign = 8 * c < 2 * a.rope_half ? 1.0f : 0.0f;
+  } else if (8 * c < a.rope_half) {
+    i0 = 8 * c;
+    pc = c + a.pair_stride / 8;
+    sign = -1.0f;
+  } else if (8 * c >= a.pair_stride && 8 * c < a.pair_stride + a.rope_half) {
+    i0 = 8 * c - a.pair_stride;
+    pc = c - a.pair_stride / 8;
+    sign = 1.0f;
+  }
+  float co[8], si[8];
+  if (sign != 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = a.pair_stride == 0 ? i0 + (e >> 1) : i0 + e;
+      const double turns = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189533577);
+      const float t = (float)(turns - __builtin_rint(turns));
+      co[e] = a.mscale * __builtin_amdgcn_cosf(t);
+      si[e] = a.mscale * __builtin_amdgcn_sinf(t);
+      if (a.pair_stride == 0) si[e] = (e & 1) ? si[e] : -si[e];
+      else si[e] *= sign;
+    }
+  }
+
+  RopeHead h[IT];
+  v4u x[IT], y[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int head = (group * IT + it) * HPW + sub;
+    RopeHead& r = h[it];
+    r.on = head < heads;
+    r.turn = sign != 0.0f;
+    if (head < a.num_q) {
+      r.src = a.q + (int64_t)tok * a.q_stride + (int64_t)head * HD;
+      r.dst = a.q_out + (int64_t)tok * a.q_out_stride + (int64_t)head * HD;
+      r.gain = a.q_norm;
+      r.norm = a.q_norm != nullptr;
+    } else {
+      const bool is_k = head < a.num_q + a.num_kv;
+      const int kv = head - a.num_q - (is_k ? 0 : a.num_kv);
+      r.src = is_k ? a.k + (int64_t)tok * a.k_stride + (int64_t)kv * HD
+                   : a.v + (int64_t)tok * a.v_stride + (int64_t)kv * HD;
+      r.dst = slot < 0 ? nullptr
+                       : (is_k ? a.k_cache : a.v_cache) + (slot * a.num_kv + kv) * (int64_t)HD;
+      r.gain = is_k ? a.k_norm : nullptr;
+      r.norm = is_k ? a.k_norm != nullptr : a.norm_v != 0;
+      r.turn = r.turn && is_k;
+    }
+    x[it] = y[it] = v4u{0, 0, 0, 0};
+    if (r.on) {
+      x[it] = *reinterpret_cast<const v4u*>(r.src + 8 * c);
+      y[it] = x[it];
+      if (r.turn && pc != c) y[it] = *reinterpret_cast<const v4u*>(r.src + 8 * pc);
+    }
+  }
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const RopeHead& r = h[it];
+    float v[8], w[8];
+    unpack8<T>(x[it], v);
+    unpack8<T>(y[it], w);
+    float ssq = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ssq = fmaf(v[e], v[e], ssq);
+#pragma unroll
+    for (int d = 1; d < LPH; d <<= 1) ssq += __shfl_xor(ssq, d);
+    if (!r.on || !r.dst) continue;
+    if (r.norm) {
+      const float inv = a.sqrt_n / __builtin_sqrtf(ssq + a.n_eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= inv, w[e] *= inv;
+      if (r.gain) {
+        float g[8], gp[8];
+        unpack8<T>(*reinterpret_cast<const v4u*>(r.gain + 8 * c), g);
+        unpack8<T>(*reinterpret_cast<const v4u*>(r.gain + 8 * pc), gp);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= g[e], w[e] *= gp[e];
+      }
+    }
+    v4u out;
+    if (r.turn) {
+      float o[8];
+      if (a.pair_stride == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e ^ 1], si[e], v[e] * co[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(w[e], si[e], v[e] * co[e]);
+      }
+      out = pack8<T>(o);
+    } else {
+      out = r.norm ? pack8<T>(v) : x[it];
+    }
+    *reinterpret_cast<v4u*>(r.dst + 8 * c) = out;
+  }
+}
+
+template <typename T, int LPH>
+hipError_t launch(const RopeArgs& a, hipStream_t st) {
+  constexpr int HPW = 64 / LPH;
+  const int heads = a.num_q + 2 * a.num_kv;
+  const int64_t waves = (int64_t)a.num_tokens * ((heads + HPW - 1) / HPW);
+  const int64_t blocks = (waves + 3) / 4;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  k_rope_append<T, LPH, 1><<<(int)blocks, 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_hd(const RopeArgs& a, int head_dim, hipStream_t st) {
+  switch (head_dim) {
+    case 64: return launch<T, 8>(a, st);
+    case 128: return launch<T, 16>(a, st);
+    case 256: return launch<T, 32>(a, st);
+    default: return launch<T, 64>(a, st);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_rope_append(const RopeArgs& a, int head_dim, bool f16, hipStream_t st) {
+  return f16 ? launch_hd<F16>(a, head_dim, st) : launch_hd<Bf16>(a, head_dim, st);
+}
+
+}  // namespace bq
