@@ -784,6 +784,8 @@ def attention(q_i8, qi_bias, f_q, k_cache, k_scale, v_cache, v_scale, runs, base
 # paged 16-bit cache and beams
 # --------------------------------------------------------------------------
 _DTYPES = {torch.float16: 5, torch.float32: 9, torch.bfloat16: 6}  # BQ_DT_*
+# the current stream's handle without a torch.cuda.Stream object around it (2.6 us each)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _half(*tensors):
@@ -798,12 +800,18 @@ def _half(*tensors):
 
 
 def _here(*tensors):
-    """Every tensor on the current device, whose current stream the call takes."""
+    """Every tensor on the current device -> the raw handle of its current stream,
+    on which the call launches."""
     dev = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:  # -1 on the host
             raise ValueError(f"libbq launches on the current device cuda:{dev}; got a tensor on "
                              f"{t.device}")
+    return _raw_stream(dev)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t: torch.Tensor, width: int):
@@ -823,11 +831,22 @@ def _table(base_rows: torch.Tensor):
 
 
 def _flat(t: torch.Tensor, dtype, n: int, name: str):
-    """A contiguous [n] tensor (of any shape with n values)."""
-    _dev(t, dtype)
-    if t.numel() != n:
-        raise ValueError(f"{name}: expected {n} values, got {tuple(t.shape)}")
+    """A contiguous tensor of n values (its device is _here's to check)."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous values, got {tuple(t.shape)}")
     return t
+
+
+def _caches(k_cache, v_cache, width: int):
+    """The rows of two contiguous caches [slots, width]."""
+    shape = k_cache.shape
+    if (len(shape) != 2 or shape[1] != width or v_cache.shape != shape or
+            not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        raise ValueError(f"caches: expected contiguous [slots, {width}] twice, got "
+                         f"{tuple(shape)} and {tuple(v_cache.shape)}")
+    return shape[0]
 
 
 def rope_frequencies(rope_half: int, base: float = 10000.0, factor: float = 1.0,
@@ -869,37 +888,35 @@ def rope_append(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, num_q
     parts of a wider buffer.  inv_freq f32 [rope_half] or None (no rotation);
     pair_stride None: rope_half (pairs by halves), 0: neighbours."""
     dt = _half(q, k, v, k_cache, v_cache, q_norm, k_norm, out)
-    _here(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, seq_ids, q_norm, k_norm, out)
+    st = _here(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, seq_ids, q_norm, k_norm, out)
     T, kw = q.shape[0], num_kv * head_dim
     qs, ks, vs = _rows(q, num_q * head_dim), _rows(k, kw), _rows(v, kw)
     if k.shape[0] != T or v.shape[0] != T:
         raise ValueError(f"rope_append: {T} rows of q, {k.shape[0]} of k, {v.shape[0]} of v")
-    for c in (k_cache, v_cache):
-        _dev(c)
-        if c.dim() != 2 or c.shape[1] != kw or c.shape[0] != k_cache.shape[0]:
-            raise ValueError(f"caches: expected [slots, {kw}] twice, got {tuple(k_cache.shape)} and "
-                             f"{tuple(v_cache.shape)}")
+    slots = _caches(k_cache, v_cache, kw)
     _flat(positions, torch.int32, T, "positions")
     if seq_ids is not None:
         _flat(seq_ids, torch.int32, T, "seq_ids")
     for g in (q_norm, k_norm):
         if g is not None:
-            _flat(g, None, head_dim, "gain")
+            _flat(g, q.dtype, head_dim, "gain")
     half = 0 if inv_freq is None else _dev(inv_freq, torch.float32).numel()
     n, width = _table(base_rows)
     if sqrt_n is None or n_eps is None:
         sqrt_n, n_eps = head_dim ** 0.5, head_dim * 1e-6
     if out is None:
         out = torch.empty((T, num_q * head_dim), dtype=q.dtype, device=q.device)
-    os_ = _rows(out, num_q * head_dim)
-    if out.shape[0] != T:
-        raise ValueError(f"out: expected {T} rows, got {out.shape[0]}")
+        os_ = num_q * head_dim
+    else:
+        os_ = _rows(out, num_q * head_dim)
+        if out.shape[0] != T:
+            raise ValueError(f"out: expected {T} rows, got {out.shape[0]}")
     _check(_lib.bq_rope_append(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, _p(q_norm), _p(k_norm), int(norm_v),
-        sqrt_n, n_eps, _p(inv_freq), half, half if pair_stride is None else pair_stride, mscale,
-        positions.data_ptr(), _p(seq_ids), base_rows.data_ptr(), n, width, page_shift,
-        k_cache.shape[0], out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), num_q,
-        num_kv, head_dim, dt, T, _stream()))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, _ptr(q_norm), _ptr(k_norm), int(norm_v),
+        sqrt_n, n_eps, _ptr(inv_freq), half, half if pair_stride is None else pair_stride, mscale,
+        positions.data_ptr(), _ptr(seq_ids), base_rows.data_ptr(), n, width, page_shift,
+        slots, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), num_q,
+        num_kv, head_dim, dt, T, st))
     return out
 
 
@@ -924,14 +941,10 @@ def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv:
     position among them.  max_kv_len sizes the splits (None: the table's);
     scale None: head_dim ** -0.5; lse: f32 [S, num_q] to fill."""
     dt = _half(q, k_cache, v_cache, out)
-    _here(q, k_cache, v_cache, base_rows, kv_lens, workspace, out, lse)
+    st = _here(q, k_cache, v_cache, base_rows, kv_lens, workspace, out, lse)
     S, kw = q.shape[0], num_kv * head_dim
     qs = _rows(q, num_q * head_dim)
-    for c in (k_cache, v_cache):
-        _dev(c)
-        if c.dim() != 2 or c.shape[1] != kw or c.shape[0] != k_cache.shape[0]:
-            raise ValueError(f"caches: expected [slots, {kw}] twice, got {tuple(k_cache.shape)} and "
-                             f"{tuple(v_cache.shape)}")
+    slots = _caches(k_cache, v_cache, kw)
     n, width = _table(base_rows)
     if n < S:
         raise ValueError(f"base_rows: {n} rows for {S} sequences")
@@ -944,32 +957,41 @@ def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv:
         workspace = paged_attention_workspace(S, num_q, head_dim, s_max, q.device)
     if out is None:
         out = torch.empty((S, num_q * head_dim), dtype=q.dtype, device=q.device)
-    _flat(out, None, S * num_q * head_dim, "out")
+    else:
+        _flat(out, q.dtype, S * num_q * head_dim, "out")
     if lse is not None:
         _flat(lse, torch.float32, S * num_q, "lse")
     _check(_lib.bq_paged_attention(
-        q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
-        base_rows.data_ptr(), width, page_shift, kv_lens.data_ptr(), out.data_ptr(), _p(lse), S,
+        q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), slots,
+        base_rows.data_ptr(), width, page_shift, kv_lens.data_ptr(), out.data_ptr(), _ptr(lse), S,
         num_q, num_kv, head_dim, window, head_dim ** -0.5 if scale is None else scale, softcap, dt,
-        max_kv_len, s_max, _p(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()))
+        max_kv_len, s_max, _ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), st))
     return out
 
 
-class _CacheArray(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("row_bytes", C.c_int64)]
+class CacheArrays:
+    """A paged cache's arrays ([slots, ...] each, contiguous) with the host table that
+    cache_reorder and cache_compact pass on: built once by a program that keeps its
+    cache, or by each call that is given a list."""
+
+    def __init__(self, arrays, slots: int):
+        self.arrays, self.slots, table = list(arrays), slots, []
+        for i, a in enumerate(self.arrays):
+            n = a.numel()
+            if a.dim() < 1 or a.shape[0] != slots or n == 0 or not a.is_contiguous():
+                raise ValueError(f"array {i}: expected {slots} contiguous rows, got "
+                                 f"{tuple(a.shape)}")
+            table += (a.data_ptr(), n // slots * a.element_size())
+        self.table = (C.c_int64 * max(len(table), 1))(*table)  # bq_cache_array pairs
 
 
 def _cache_arrays(arrays, slots: int):
-    """The host table of a cache's arrays ([slots, ...] each) for one call."""
-    table = (_CacheArray * max(len(arrays), 1))()
-    for i, a in enumerate(arrays):
-        _dev(a)
-        if a.dim() < 1 or a.shape[0] != slots or a.numel() == 0:
-            raise ValueError(f"array {i}: expected {slots} rows, got {tuple(a.shape)}")
-        table[i].data = a.data_ptr()
-        table[i].row_bytes = a.numel() // slots * a.element_size()
-    return table
+    if not isinstance(arrays, CacheArrays):
+        return CacheArrays(arrays, slots)
+    if arrays.slots != slots:
+        raise ValueError(f"arrays have {arrays.slots} rows, the pool {slots}")
+    return arrays
 
 
 def cache_reorder(arrays, base_rows, lens, refs, parents, page_shift: int, grow=None,
@@ -977,44 +999,47 @@ def cache_reorder(arrays, base_rows, lens, refs, parents, page_shift: int, grow=
     """bq_cache_reorder: sequence i goes on as old sequence parents[i] (-1: empty)
     with room for grow[i] more positions; base_rows [N, pages], lens [N], refs
     [pool] change in place, written pages are copied in every array ([pool <<
-    page_shift, ...]) -> info int32 [4] (fresh, copied, missing, 0)."""
-    _here(base_rows, lens, refs, parents, grow, workspace, info, *arrays)
+    page_shift, ...], a list or CacheArrays) -> info int32 [4] (fresh, copied, missing,
+    0)."""
     n, width = _table(base_rows)
     _flat(lens, torch.int32, n, "lens")
     _flat(parents, torch.int32, n, "parents")
     if grow is not None:
         _flat(grow, torch.int32, n, "grow")
     pool = _dev(refs, torch.int32).numel()
-    table = _cache_arrays(arrays, pool << page_shift)
+    arrays = _cache_arrays(arrays, pool << page_shift)
+    st = _here(base_rows, lens, refs, parents, grow, workspace, info, *arrays.arrays)
     if workspace is None:
         workspace = torch.empty(int(_lib.bq_cache_reorder_workspace_size(n)), dtype=torch.uint8,
                                 device=base_rows.device)
     if info is None:
         info = torch.empty(4, dtype=torch.int32, device=base_rows.device)
-    _flat(info, torch.int32, 4, "info")
-    _check(_lib.bq_cache_reorder(table, len(arrays), base_rows.data_ptr(), lens.data_ptr(),
-                                 refs.data_ptr(), parents.data_ptr(), _p(grow), n, width,
+    else:
+        _flat(info, torch.int32, 4, "info")
+    _check(_lib.bq_cache_reorder(arrays.table, len(arrays.arrays), base_rows.data_ptr(), lens.data_ptr(),
+                                 refs.data_ptr(), parents.data_ptr(), _ptr(grow), n, width,
                                  page_shift, pool, info.data_ptr(), workspace.data_ptr(),
-                                 workspace.numel() * workspace.element_size(), _stream()))
+                                 workspace.numel() * workspace.element_size(), st))
     return info
 
 
 def cache_compact(arrays, base_rows, refs, page_shift: int, workspace=None, info=None):
     """bq_cache_compact: the held pages move below their number; base_rows, refs
     and every array change in place -> info int32 [4] (held, moved, 0, 0)."""
-    _here(base_rows, refs, workspace, info, *arrays)
     n, width = _table(base_rows)
     pool = _dev(refs, torch.int32).numel()
-    table = _cache_arrays(arrays, pool << page_shift)
+    arrays = _cache_arrays(arrays, pool << page_shift)
+    st = _here(base_rows, refs, workspace, info, *arrays.arrays)
     if workspace is None:
         workspace = torch.empty(int(_lib.bq_cache_compact_workspace_size(pool)),
                                 dtype=torch.uint8, device=base_rows.device)
     if info is None:
         info = torch.empty(4, dtype=torch.int32, device=base_rows.device)
-    _flat(info, torch.int32, 4, "info")
-    _check(_lib.bq_cache_compact(table, len(arrays), base_rows.data_ptr(), refs.data_ptr(), n,
+    else:
+        _flat(info, torch.int32, 4, "info")
+    _check(_lib.bq_cache_compact(arrays.table, len(arrays.arrays), base_rows.data_ptr(), refs.data_ptr(), n,
                                  width, page_shift, pool, info.data_ptr(), workspace.data_ptr(),
-                                 workspace.numel() * workspace.element_size(), _stream()))
+                                 workspace.numel() * workspace.element_size(), st))
     return info
 
 
@@ -1029,7 +1054,7 @@ def beam_select(logits, scores, n: int | None = None, finished=None, eos_id: int
     _dev(scores, torch.float32)
     if scores.dim() != 2 or logits.dim() != 2:
         raise ValueError("scores: [requests, beams], logits: [requests * beams, vocab]")
-    _here(logits, scores, finished, workspace)
+    st = _here(logits, scores, finished, workspace)
     b, k = scores.shape
     rows, vocab = logits.shape
     if rows != b * k:
@@ -1050,14 +1075,15 @@ def beam_select(logits, scores, n: int | None = None, finished=None, eos_id: int
                torch.empty((b, n), dtype=torch.int32, device=d))
         if finished is not None:
             out += (torch.empty((b, n), dtype=torch.uint8, device=d),)
-    for t, dt in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8)):
-        _flat(t, dt, b * n, "out")
-    _here(*out)
+    else:
+        for t, dt in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8)):
+            _flat(t, dt, b * n, "out")
+        _here(*out)
     _check(_lib.bq_beam_select(logits.data_ptr(), stride, _DTYPES[logits.dtype],
-                               scores.data_ptr(), _p(finished), b, k, vocab, n, eos_id,
+                               scores.data_ptr(), _ptr(finished), b, k, vocab, n, eos_id,
                                out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
                                out[3].data_ptr() if len(out) > 3 else None, workspace.data_ptr(),
-                               workspace.numel() * workspace.element_size(), _stream()))
+                               workspace.numel() * workspace.element_size(), st))
     return out
 
 

@@ -8,9 +8,8 @@
 // A page's reference count is the number of table entries (of any table over the
 // pool) that hold it; 0 is free.  A reorder, in terms of whole tables:
 //   1. k_reorder_tables: every sequence takes its parent's entries (in place: a
-//      workgroup owns all rows of a few columns), and the counts follow: an old
-//      entry counts once for each child that keeps it instead of once.
-//   2. k_reorder_plan (one workgroup): the page a sequence writes next has to be
+//      workgroup owns all rows of a few columns), and the counts follow.
+//   2. k_reorder_plan (one workgroup, which does small tables too): the page a sequence writes next has to be
 //      its own.  Of the sequences on one such page, in their order, all but the
 //      last leave it for a fresh page while anyone else holds it; fresh pages are
 //      the lowest free numbers in the order (sequence, page).
@@ -27,7 +26,9 @@ namespace bq {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kTileEntries = 8192;  // LDS entries of k_reorder_tables (32 KiB)
+constexpr int kTableThreads = 512;
+constexpr int kTileEntries = 1024;  // table entries of a k_reorder_tables workgroup
+constexpr int64_t kOneBytes = 56000;  // tables and counts that k_reorder_plan<true> keeps in LDS
 
 struct CopyItem {
   int32_t src, dst, rows, pad;
@@ -38,47 +39,6 @@ struct CopyList {
   int32_t count, pad[3];
   CopyItem item[1];
 };
-
-__global__ __launch_bounds__(256) void k_reorder_tables(ReorderArgs a, int cols) {
-  extern __shared__ int32_t lds[];
-  int32_t* tile = lds;                               // [num_seqs][cols] page numbers
-  int32_t* shares = lds + (size_t)a.num_seqs * cols;  // children of each sequence
-  int32_t* writes = shares + a.num_seqs;              // of these, with a page to write
-  const int j0 = blockIdx.x * cols, n = a.num_seqs;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) shares[i] = writes[i] = 0;
-  for (int e = threadIdx.x; e < n * cols; e += blockDim.x) {
-    const int s = e / cols, j = j0 + e % cols;
-    tile[e] = j < a.max_pages
-                  ? page_number(a.base_rows[(int64_t)s * a.max_pages + j], a.page_shift, a.num_pages)
-                  : -1;
-  }
-  __syncthreads();
-  auto plan_of = [&](int i) {
-    const int p = a.parents[i];
-    return seq_plan(p, n, p >= 0 && p < n ? a.lens[p] : 0, a.grow ? a.grow[i] : 0, a.max_pages,
-                    a.page_shift);
-  };
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const SeqPlan s = plan_of(i);
-    if (s.parent >= 0) {
-      atomicAdd(&shares[s.parent], 1);
-      if (s.full < s.end) atomicAdd(&writes[s.parent], 1);
-    }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < n * cols; e += blockDim.x) {
-    const int s = e / cols, j = j0 + e % cols;
-    if (j >= a.max_pages) continue;
-    if (tile[e] >= 0) {  // the old entry
-      const SeqPlan own = seq_plan(s, n, a.lens[s], 0, a.max_pages, a.page_shift);
-      const int d = (j < own.full ? shares[s] : j == own.full ? writes[s] : 0) - 1;
-      if (d) atomicAdd(&a.refs[tile[e]], d);
-    }
-    const SeqPlan p = plan_of(s);  // the new one
-    const int page = seq_keeps(p, j) ? tile[p.parent * cols + e % cols] : -1;
-    a.base_rows[(int64_t)s * a.max_pages + j] = page >= 0 ? page << a.page_shift : -1;
-  }
-}
 
 // inclusive scan over the workgroup; total in *sum
 __device__ inline int block_scan(int v, int* wsum, int* sum) {
@@ -98,87 +58,179 @@ __device__ inline int block_scan(int v, int* wsum, int* sum) {
   return inc + before;
 }
 
+// What a workgroup keeps in LDS of each sequence: where it comes from, and how many
+// go on from it.
+struct SeqLds {
+  int32_t parent, len, full, end;  // SeqPlan
+  int32_t own_full;                // whole pages it had itself
+  int32_t shares, writes;          // its children, and those with a page to write
+};
+
+__device__ inline SeqPlan plan_of(const SeqLds& q) {
+  return SeqPlan{q.parent, q.len, q.full, q.end};
+}
+
+// every sequence's plan; to be followed by a barrier and count_children
+__device__ inline void load_seqs(const ReorderArgs& a, SeqLds* seq, int threads) {
+  for (int i = threadIdx.x; i < a.num_seqs; i += threads) {
+    const int p = a.parents[i];
+    const SeqPlan s = seq_plan(p, a.num_seqs, p >= 0 && p < a.num_seqs ? a.lens[p] : 0,
+                               a.grow ? a.grow[i] : 0, a.max_pages, a.page_shift);
+    const SeqPlan own = seq_plan(i, a.num_seqs, a.lens[i], 0, a.max_pages, a.page_shift);
+    seq[i] = SeqLds{s.parent, s.len, s.full, s.end, own.full, 0, 0};
+  }
+}
+
+__device__ inline void count_children(const ReorderArgs& a, SeqLds* seq, int threads) {
+  for (int i = threadIdx.x; i < a.num_seqs; i += threads) {
+    const int p = seq[i].parent;
+    if (p >= 0) {
+      atomicAdd(&seq[p].shares, 1);
+      if (seq[i].full < seq[i].end) atomicAdd(&seq[p].writes, 1);
+    }
+  }
+}
+
+// columns [j0, j0 + width) of the tables: old page numbers to LDS ...
+__device__ inline void load_tile(const ReorderArgs& a, int32_t* tile, int j0, int width,
+                                 int threads) {
+  for (int e = threadIdx.x; e < a.num_seqs * width; e += threads) {
+    const int s = e / width;
+    tile[e] = page_number(a.base_rows[(int64_t)s * a.max_pages + j0 + (e - s * width)], a.page_shift,
+                          a.num_pages);
+  }
+}
+
+// ... and the new entries and counts from there: an old entry counts once for each
+// child that keeps it instead of once
+__device__ inline void store_tile(const ReorderArgs& a, int32_t* refs, const SeqLds* seq,
+                                  const int32_t* tile, int j0, int width, int threads) {
+  for (int e = threadIdx.x; e < a.num_seqs * width; e += threads) {
+    const int s = e / width, c = e - s * width, j = j0 + c;
+    const SeqLds q = seq[s];
+    if (tile[e] >= 0) {
+      const int d = (j < q.own_full ? q.shares : j == q.own_full ? q.writes : 0) - 1;
+      if (d) atomicAdd(&refs[tile[e]], d);
+    }
+    const int page = seq_keeps(plan_of(q), j) ? tile[q.parent * width + c] : -1;
+    a.base_rows[(int64_t)s * a.max_pages + j] = page >= 0 ? page << a.page_shift : -1;
+  }
+}
+
+__global__ __launch_bounds__(kTableThreads) void k_reorder_tables(ReorderArgs a, int cols) {
+  extern __shared__ int32_t lds[];
+  SeqLds* seq = reinterpret_cast<SeqLds*>(lds);                     // [num_seqs]
+  int32_t* tile = lds + (size_t)a.num_seqs * (sizeof(SeqLds) / 4);  // [num_seqs][width]
+  const int j0 = blockIdx.x * cols, width = min(cols, a.max_pages - j0);
+  load_seqs(a, seq, kTableThreads);
+  load_tile(a, tile, j0, width, kTableThreads);
+  __syncthreads();
+  count_children(a, seq, kTableThreads);
+  __syncthreads();
+  store_tile(a, a.refs, seq, tile, j0, width, kTableThreads);
+}
+
+// ONE: the whole reorder's bookkeeping, with tables and counts in LDS; else what
+// k_reorder_tables leaves to do.
+template <bool ONE>
 __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
+  extern __shared__ __align__(16) int32_t lds[];
+  const int pages4 = (a.num_pages + 3) & ~3;
+  int32_t* refs = ONE ? lds : a.refs;                               // [num_pages]
+  SeqLds* seq = reinterpret_cast<SeqLds*>(lds + (ONE ? pages4 : 0));  // [num_seqs]
+  int32_t* tile = reinterpret_cast<int32_t*>(seq + a.num_seqs);     // ONE: [num_seqs][max_pages]
   __shared__ int wsum[kPlanThreads / 64];
-  __shared__ int32_t last[kMaxCacheSeqs], offset[kMaxCacheSeqs + 1];
-  __shared__ int ncopy, nfree;
+  __shared__ __align__(16) int32_t last[kMaxCacheSeqs];
+  __shared__ int32_t offset[kMaxCacheSeqs + 1];
+  __shared__ int ncopy;
   CopyList* list = static_cast<CopyList*>(a.workspace);
   const int n = a.num_seqs, i = threadIdx.x;
+  if (i == 0) ncopy = 0;
+  load_seqs(a, seq, kPlanThreads);
+  if constexpr (ONE) {
+    load_tile(a, tile, 0, a.max_pages, kPlanThreads);
+    for (int q = i; q < pages4; q += kPlanThreads) refs[q] = q < a.num_pages ? a.refs[q] : -1;
+    __syncthreads();
+    count_children(a, seq, kPlanThreads);
+    __syncthreads();
+    store_tile(a, refs, seq, tile, 0, a.max_pages, kPlanThreads);
+  }
   SeqPlan p{};
   int page = -1;
   if (i < n) {
-    const int par = a.parents[i];
-    p = seq_plan(par, n, par >= 0 && par < n ? a.lens[par] : 0, a.grow ? a.grow[i] : 0,
-                 a.max_pages, a.page_shift);
-    if (p.full < p.end)
-      page = page_number(a.base_rows[(int64_t)i * a.max_pages + p.full], a.page_shift, a.num_pages);
-    last[i] = page;
+    p = plan_of(seq[i]);
+    if (p.full < p.end) {
+      if constexpr (ONE)
+        page = p.parent >= 0 ? tile[p.parent * a.max_pages + p.full] : -1;
+      else
+        page = page_number(a.base_rows[(int64_t)i * a.max_pages + p.full], a.page_shift,
+                           a.num_pages);
+    }
   }
-  if (i == 0) ncopy = nfree = 0;
-  __syncthreads();
-  if (i < n) a.lens[i] = p.len;  // every length has been read
+  last[i] = page;
+  __syncthreads();  // every length has been read, every count changed
+  if (i < n) a.lens[i] = p.len;
   bool leaves = false;
   if (page >= 0) {
     int earlier = 0;
-    for (int k = 0; k < i; ++k) earlier += last[k] == page;
-    leaves = a.refs[page] - earlier > 1;
+    for (int k = 0; k < (i & ~3); k += 4) {
+      const v4i l = *reinterpret_cast<const v4i*>(last + k);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) earlier += l[u] == page;
+    }
+    for (int k = i & ~3; k < i; ++k) earlier += last[k] == page;
+    leaves = refs[page] - earlier > 1;
   }
-  int fresh = p.end - p.full;
-  if (i >= n) fresh = 0;
+  int fresh = i < n ? p.end - p.full : 0;
   if (page >= 0 && !leaves) --fresh;
   int total;
   const int incl = block_scan(fresh, wsum, &total);
   if (i < n) offset[i] = incl - fresh;
   if (i == 0) offset[n] = total;
-  if (leaves) atomicAdd(&a.refs[page], -1);  // it stays above 0: the last one keeps it
+  if (leaves) atomicAdd(&refs[page], -1);  // it stays above 0: the last one keeps it
   __syncthreads();
 
-  // the first `total` free pages, lowest numbers first
-  int got = 0;
-  for (int base = 0; base < a.num_pages && got < total; base += kPlanThreads) {
-    const int q = base + i;
-    const int free_ = q < a.num_pages && a.refs[q] == 0;
-    int found;
-    const int k = got + block_scan(free_, wsum, &found) - free_;
-    if (free_ && k < total) {
-      int lo = 0, hi = n - 1;  // the sequence: the last one with offset <= k
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (offset[mid] <= k) lo = mid;
-        else hi = mid - 1;
-      }
-      const int par = a.parents[lo];
-      // its length is in lens already
-      const SeqPlan s = seq_plan(par >= 0 && par < n ? 0 : -1, n, a.lens[lo], a.grow ? a.grow[lo] : 0,
-                                 a.max_pages, a.page_shift);
-      const int count = offset[lo + 1] - offset[lo];
-      const int j = s.end - count + (k - offset[lo]);
-      a.refs[q] = 1;
-      a.base_rows[(int64_t)lo * a.max_pages + j] = q << a.page_shift;
-      const int rows = s.len & ((1 << a.page_shift) - 1);
-      if (j == s.full && last[lo] >= 0 && rows) {
-        const int at = atomicAdd(&ncopy, 1);
-        list->item[at] = CopyItem{last[lo] << a.page_shift, q << a.page_shift, rows, 0};
-      }
-    }
-    got += found;
-  }
-  if (got > total) got = total;
-  // entries that found no page
-  for (int k = got + i; k < total; k += kPlanThreads) {
-    int lo = 0, hi = n - 1;
+  // the k-th page that is wanted: a sequence's, found by bisection of the offsets
+  auto give = [&](int k, int page_) {
+    int lo = 0, hi = n - 1;  // the last sequence with offset <= k
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (offset[mid] <= k) lo = mid;
       else hi = mid - 1;
     }
-    const int par = a.parents[lo];
-    const SeqPlan s = seq_plan(par >= 0 && par < n ? 0 : -1, n, a.lens[lo], a.grow ? a.grow[lo] : 0,
-                               a.max_pages, a.page_shift);
-    const int count = offset[lo + 1] - offset[lo];
-    a.base_rows[(int64_t)lo * a.max_pages + s.end - count + (k - offset[lo])] = -1;
+    const SeqPlan s = plan_of(seq[lo]);
+    const int j = s.end - (offset[lo + 1] - k);
+    a.base_rows[(int64_t)lo * a.max_pages + j] = page_ >= 0 ? page_ << a.page_shift : -1;
+    const int rows = s.len & ((1 << a.page_shift) - 1);
+    if (page_ >= 0 && j == s.full && last[lo] >= 0 && rows)
+      list->item[atomicAdd(&ncopy, 1)] =
+          CopyItem{last[lo] << a.page_shift, page_ << a.page_shift, rows, 0};
+  };
+  // the first `total` free pages, lowest numbers first, four a thread
+  int got = 0;
+  for (int base = 0; base < a.num_pages && got < total; base += 4 * kPlanThreads) {
+    const int q = base + 4 * i;
+    int free_ = 0, found;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (q + u < a.num_pages && refs[q + u] == 0) free_ |= 1 << u;
+    int k = got + block_scan(__popc(free_), wsum, &found) - __popc(free_);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (free_ >> u & 1) {
+        if (k < total) {
+          refs[q + u] = 1;
+          give(k, q + u);
+        }
+        ++k;
+      }
+    got += found;
   }
+  if (got > total) got = total;
+  for (int k = got + i; k < total; k += kPlanThreads) give(k, -1);  // no page left for these
   __syncthreads();
+  if constexpr (ONE)
+    for (int q = i; q < a.num_pages; q += kPlanThreads) a.refs[q] = refs[q];
   if (i == 0) {
     list->count = ncopy;
     a.info[0] = got;
@@ -195,23 +247,33 @@ __global__ __launch_bounds__(kPlanThreads) void k_compact_plan(CompactArgs a) {
   const int i = threadIdx.x;
   CopyList* list = static_cast<CopyList*>(a.workspace);
   int32_t* to = reinterpret_cast<int32_t*>(list->item + (a.num_pages / 2 + 1));
+  auto held4 = [&](int q) {  // which of four pages are held, as bits
+    int m = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (q + u < a.num_pages && a.refs[q + u] != 0) m |= 1 << u;
+    return m;
+  };
   int mine = 0, live;
-  for (int q = i; q < a.num_pages; q += kPlanThreads) mine += a.refs[q] != 0;
+  for (int q = 4 * i; q < a.num_pages; q += 4 * kPlanThreads) mine += __popc(held4(q));
   block_scan(mine, wsum, &live);
   int holes = 0, movers = 0;
-  for (int base = 0; base < a.num_pages; base += kPlanThreads) {
-    const int q = base + i;
-    const bool in = q < a.num_pages;
-    const bool held = in && a.refs[q] != 0;
-    const int hole = in && !held && q < live, mover = held && q >= live;
-    int nh, nm;
-    const int kh = holes + block_scan(hole, wsum, &nh) - hole;
-    const int km = movers + block_scan(mover, wsum, &nm) - mover;
-    if (hole) list->item[kh].dst = q;
-    if (mover) list->item[km].src = q;
-    if (in) to[q] = q;
-    holes += nh;
-    movers += nm;
+  for (int base = 0; base < a.num_pages; base += 4 * kPlanThreads) {
+    const int q = base + 4 * i, held = held4(q);
+    const int in = min(max(a.num_pages - q, 0), 4), low = min(max(live - q, 0), 4);
+    const int hole = ~held & ((1 << low) - 1), mover = held & ~((1 << low) - 1);
+    int both;  // at most 4096 of each: two counts in one scan
+    const int mineboth = __popc(hole) | __popc(mover) << 16;
+    const int before = block_scan(mineboth, wsum, &both) - mineboth;
+    int kh = holes + (before & 0xFFFF), km = movers + (before >> 16);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (hole >> u & 1) list->item[kh++].dst = q + u;
+      if (mover >> u & 1) list->item[km++].src = q + u;
+      if (u < in) to[q + u] = q + u;
+    }
+    holes += both & 0xFFFF;
+    movers += both >> 16;
   }
   __syncthreads();
   for (int k = i; k < movers; k += kPlanThreads) {
@@ -229,37 +291,49 @@ __global__ __launch_bounds__(kPlanThreads) void k_compact_plan(CompactArgs a) {
   }
 }
 
-__global__ __launch_bounds__(256) void k_compact_tables(CompactArgs a) {
-  const CopyList* list = static_cast<const CopyList*>(a.workspace);
-  const int32_t* to = reinterpret_cast<const int32_t*>(list->item + (a.num_pages / 2 + 1));
-  if (list->count == 0) return;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= (int64_t)a.num_seqs * a.max_pages) return;
-  const int page = page_number(a.base_rows[e], a.page_shift, a.num_pages);
-  if (page >= 0) a.base_rows[e] = to[page] << a.page_shift;
-}
-
 // Rows of pages in every array: a work item is kSegment bytes of one copy of one
-// array.
+// array, eight 16-byte loads a thread ahead of its stores.
 constexpr int64_t kSegment = 32768;
 
 template <typename W>
 __device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
-  const int64_t n = bytes / (int64_t)sizeof(W);
-  for (int64_t k = threadIdx.x; k < n; k += 256)
-    reinterpret_cast<W*>(d)[k] = reinterpret_cast<const W*>(s)[k];
+  constexpr int U = 8;
+  const int n = (int)(bytes / (int64_t)sizeof(W));
+  W* dw = reinterpret_cast<W*>(d);
+  const W* sw = reinterpret_cast<const W*>(s);
+  for (int k = threadIdx.x; k < n; k += 256 * U) {
+    W w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u * 256 < n) w[u] = sw[k + u * 256];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u * 256 < n) dw[k + u * 256] = w[u];
+  }
 }
 
+// The first `table_blocks` workgroups (compaction) carry the tables over to the new
+// page numbers, the others copy.
 __global__ __launch_bounds__(256) void k_cache_copy(CacheArrays arrays, const void* workspace,
-                                                    int segments) {
+                                                    int segments, CompactArgs t, int table_blocks) {
   const CopyList* list = static_cast<const CopyList*>(workspace);
+  if (list->count == 0) return;
+  if (blockIdx.x < table_blocks) {
+    const int32_t* to = reinterpret_cast<const int32_t*>(list->item + (t.num_pages / 2 + 1));
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= (int64_t)t.num_seqs * t.max_pages) return;
+    const int page = page_number(t.base_rows[e], t.page_shift, t.num_pages);
+    if (page >= 0) t.base_rows[e] = to[page] << t.page_shift;
+    return;
+  }
   const int64_t per = (int64_t)arrays.n * segments, total = (int64_t)list->count * per;
-  for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-    const CopyItem it = list->item[w / per];
-    const int r = (int)(w % per);
-    const int64_t row = arrays.row_bytes[r / segments];
-    uint8_t* data = static_cast<uint8_t*>(arrays.data[r / segments]);
-    const int64_t at = (r % segments) * kSegment, bytes = (int64_t)it.rows * row;
+  for (int64_t w = blockIdx.x - table_blocks; w < total; w += gridDim.x - table_blocks) {
+    const int64_t which = w / per;
+    const CopyItem it = list->item[which];
+    const int r = (int)(w - which * per), array = r / segments;
+    const int64_t row = arrays.row_bytes[array];
+    uint8_t* data = static_cast<uint8_t*>(arrays.data[array]);
+    const int64_t at = (int64_t)(r - array * segments) * kSegment, bytes = (int64_t)it.rows * row;
     if (at >= bytes) continue;
     const int64_t len = bytes - at < kSegment ? bytes - at : kSegment;
     uint8_t* d = data + it.dst * row + at;
@@ -272,14 +346,17 @@ __global__ __launch_bounds__(256) void k_cache_copy(CacheArrays arrays, const vo
 }
 
 hipError_t launch_copy(const CacheArrays& arrays, void* workspace, int max_items, int page_shift,
-                       hipStream_t st) {
-  if (arrays.n == 0 || max_items == 0) return hipSuccess;
+                       hipStream_t st, const CompactArgs* t = nullptr) {
   int64_t most = 0;
   for (int i = 0; i < arrays.n; ++i) most = std::max(most, arrays.row_bytes[i] << page_shift);
-  const int64_t segments = (most + kSegment - 1) / kSegment;
-  if (segments * arrays.n > INT32_MAX) return hipErrorInvalidValue;
-  const int64_t items = std::min<int64_t>((int64_t)max_items * arrays.n * segments, 4096);
-  k_cache_copy<<<(int)items, 256, 0, st>>>(arrays, workspace, (int)segments);
+  const int64_t segments = std::max<int64_t>(1, (most + kSegment - 1) / kSegment);
+  const int64_t entries = t ? (int64_t)t->num_seqs * t->max_pages : 0;
+  const int64_t table_blocks = (entries + 255) / 256;
+  const int64_t copies = std::min<int64_t>((int64_t)max_items * arrays.n * segments, 4096);
+  if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
+  if (copies == 0 && table_blocks == 0) return hipSuccess;
+  k_cache_copy<<<(int)(table_blocks + std::max<int64_t>(copies, 1)), 256, 0, st>>>(
+      arrays, workspace, (int)segments, t ? *t : CompactArgs{}, (int)table_blocks);
   return hipGetLastError();
 }
 
@@ -291,27 +368,28 @@ size_t compact_workspace(int num_pages) {
 }
 
 hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays, hipStream_t st) {
-  const int cols = std::max(1, std::min(64, kTileEntries / a.num_seqs));
-  const int blocks = (a.max_pages + cols - 1) / cols;
-  const size_t lds = ((size_t)a.num_seqs * cols + 2 * (size_t)a.num_seqs) * 4;
-  k_reorder_tables<<<blocks, 256, lds, st>>>(a, cols);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  k_reorder_plan<<<1, kPlanThreads, 0, st>>>(a);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  return launch_copy(arrays, a.workspace, a.num_seqs, a.page_shift, st);
+  const size_t seqs = sizeof(SeqLds) * a.num_seqs;
+  // What fits LDS one workgroup does alone: a launch less.
+  const int64_t one = seqs + ((int64_t)a.num_seqs * a.max_pages + ((a.num_pages + 3) & ~3)) * 4;
+  if (one <= kOneBytes) {
+    k_reorder_plan<true><<<1, kPlanThreads, (size_t)one, st>>>(a);
+  } else {
+    const int cols = std::max(1, std::min(a.max_pages, kTileEntries / a.num_seqs));
+    k_reorder_tables<<<(a.max_pages + cols - 1) / cols, kTableThreads,
+                       seqs + (size_t)cols * a.num_seqs * 4, st>>>(a, cols);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_reorder_plan<false><<<1, kPlanThreads, seqs, st>>>(a);
+  }
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : launch_copy(arrays, a.workspace, a.num_seqs, a.page_shift, st);
 }
 
 hipError_t launch_cache_compact(const CompactArgs& a, const CacheArrays& arrays, hipStream_t st) {
   k_compact_plan<<<1, kPlanThreads, 0, st>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const int64_t entries = (int64_t)a.num_seqs * a.max_pages;
-  k_compact_tables<<<(int)((entries + 255) / 256), 256, 0, st>>>(a);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  return launch_copy(arrays, a.workspace, a.num_pages / 2, a.page_shift, st);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e
+                         : launch_copy(arrays, a.workspace, a.num_pages / 2, a.page_shift, st, &a);
 }
 
 }  // namespace bq

@@ -73,15 +73,22 @@ __device__ inline Range attn_range(const PagedAttnArgs& a, int seq, int split, i
   return r;
 }
 
-// HD = 512 takes 16 positions a tile: K, V, the queries and the accumulators of
-// 32 would pass the 512 registers of a lane.
+// From HD = 256 on, 16 positions a tile: K, V, the queries and the accumulators of 32
+// would pass the registers that leave room for two waves (HD = 512: for one).
 template <int HD>
 constexpr int tile_positions() {
-  return HD == 512 ? 16 : 32;
+  return HD >= 256 ? 16 : 32;
 }
 
-template <typename T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
+// Pages of fewer than 16 rows (SMALL) are looked up position by position and their
+// slots passed between lanes; larger ones once per 16 positions, with the wave's
+// address in scalar registers and the lanes' offsets the same for every tile.
+//
+// The next tile's rows are asked for as soon as the registers of this one's are free:
+// K behind the scores, V behind the value product.
+template <typename T, int HD, int NW, bool SMALL>
+__global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
+    PagedAttnArgs a) {
   constexpr int TP = tile_positions<HD>();
   constexpr int KS = HD / 32;            // steps of the score product
   constexpr int MT = TP / 16;            // groups of 16 positions
@@ -90,9 +97,10 @@ __global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
   constexpr int VW = CPL / 2;            // words of a value load
   constexpr int NP = TP / 4;             // positions per lane of the value product
   constexpr int LD = HD + 8;             // LDS row: 16 heads 32 bytes apart in the banks
+  constexpr uint32_t FULL = (uint32_t)((1ull << TP) - 1);
 
   extern __shared__ float smem[];  // acc [NW][G][LD], then m, l [NW][16] each
-  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, quad = lane >> 4;
 
   int b = blockIdx.x;
@@ -118,47 +126,75 @@ __global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
 
   const int32_t* rows = a.base_rows + (int64_t)seq * a.max_pages;
   const int64_t stride = (int64_t)a.num_kv * HD;
-  const uint16_t* kc = a.k_cache + (int64_t)kvh * HD + quad * 8;
-  const uint16_t* vc = a.v_cache + (int64_t)kvh * HD + n16 * CPL;
-
-  v4f32 o[CG][CPL];
+  const uint16_t* kc = a.k_cache + (int64_t)kvh * HD;
+  const uint16_t* vc = a.v_cache + (int64_t)kvh * HD;
+  const uint32_t koff = (uint32_t)(n16 * stride + quad * 8) * 2;
+  uint32_t voff[4];
 #pragma unroll
-  for (int i = 0; i < CG; ++i)
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) o[i][c] = v4f32{0, 0, 0, 0};
-  float m = -INFINITY, l = 0.0f;
+  for (int r = 0; r < 4; ++r) voff[r] = (uint32_t)((quad * 4 + r) * stride + n16 * CPL) * 2;
 
-  for (int t = rg.t0 + wave; t < rg.t1; t += NW) {
-    const int p0 = t * TP;
-    // slots of the tile's rows, and which of its positions take part
+  // a tile's rows: its slots (SMALL: of this lane's rows; else of the first row of each
+  // 16, the same in all lanes) and which of its positions take part
+  struct Tile {
     uint32_t ok;
-    int64_t kslot[MT], vslot[NP];
-    {
+    int32_t slot[SMALL ? MT + NP : MT];
+  };
+  auto find = [&](int t) {
+    Tile x;
+    const int p0 = t * TP;
+    if constexpr (SMALL) {
       const int p = p0 + (lane & (TP - 1));
       const bool in = p >= rg.start && p < rg.len;
       const int64_t s = in ? page_slot(rows, a.max_pages, a.page_shift, a.num_slots, p) : -1;
-      ok = (uint32_t)(__ballot(s >= 0)) & (uint32_t)((1ull << TP) - 1);
+      x.ok = (uint32_t)__ballot(s >= 0) & FULL;
       const int sl = s < 0 ? 0 : (int)s;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) kslot[i] = __shfl(sl, i * 16 + n16);
+      for (int i = 0; i < MT; ++i) x.slot[i] = __shfl(sl, i * 16 + n16);
 #pragma unroll
-      for (int j = 0; j < NP; ++j) vslot[j] = __shfl(sl, (j >> 2) * 16 + quad * 4 + (j & 3));
+      for (int j = 0; j < NP; ++j)
+        x.slot[MT + j] = __shfl(sl, (j >> 2) * 16 + quad * 4 + (j & 3));
+    } else {
+      x.ok = FULL;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int p = p0 + i * 16;
+        // past the end there may be no entry: nothing of these 16 takes part
+        const int32_t base = p < rg.len ? rows[p >> a.page_shift] : -1;
+        const bool in = page_in(base, a.page_shift, a.num_slots);
+        x.slot[i] = in ? base + (p & ((1 << a.page_shift) - 1)) : 0;
+        if (!in) x.ok &= ~(0xFFFFu << (16 * i));
+      }
+      if (p0 + TP > rg.len) x.ok &= (uint32_t)((1ull << (rg.len - p0)) - 1);
+      if (p0 < rg.start) x.ok &= ~(uint32_t)((1ull << (rg.start - p0)) - 1);
     }
-    v4u kf[MT][KS];
+    return x;
+  };
+  v4u kf[MT][KS];
+  uint32_t vf[CG][NP][VW];
+  auto load_k = [&](const Tile& x) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const uint16_t* p = kc + kslot[i] * stride;
+      const char* p;
+      if constexpr (SMALL)
+        p = reinterpret_cast<const char*>(kc + x.slot[i] * stride + quad * 8);
+      else
+        p = reinterpret_cast<const char*>(kc + x.slot[i] * stride) + koff;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[i][ks] = *reinterpret_cast<const v4u*>(p + ks * 32);
+      for (int ks = 0; ks < KS; ++ks) kf[i][ks] = *reinterpret_cast<const v4u*>(p + ks * 64);
     }
-    uint32_t vf[CG][NP][VW];
+  };
+  auto load_v = [&](const Tile& x) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const uint16_t* p = vc + vslot[j] * stride;
+      const char* p;
+      if constexpr (SMALL)
+        p = reinterpret_cast<const char*>(vc + x.slot[MT + j] * stride + n16 * CPL);
+      else
+        p = reinterpret_cast<const char*>(vc + x.slot[j >> 2] * stride) + voff[j & 3];
 #pragma unroll
       for (int i = 0; i < CG; ++i) {
         if constexpr (VW == 4) {
-          const v4u w = *reinterpret_cast<const v4u*>(p + i * 128);
+          const v4u w = *reinterpret_cast<const v4u*>(p + i * 256);
 #pragma unroll
           for (int x = 0; x < 4; ++x) vf[i][j][x] = w[x];
         } else {
@@ -168,22 +204,46 @@ __global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
         }
       }
     }
+  };
+
+  v4f32 o[CG][CPL];
+#pragma unroll
+  for (int i = 0; i < CG; ++i)
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) o[i][c] = v4f32{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  int t = rg.t0 + wave;
+  Tile cur{}, next{};
+  if (t < rg.t1) {
+    cur = find(t);
+    load_k(cur);
+    load_v(cur);
+    if (t + NW < rg.t1) next = find(t + NW);
+  }
+  for (; t < rg.t1; t += NW) {
+    const bool more = t + NW < rg.t1;
     // scores in powers of two, -inf where a position takes no part
     float x[NP];
     float mt = -INFINITY;
+    v4f32 sc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      v4f32 s = {0, 0, 0, 0};
+      sc[i] = v4f32{0, 0, 0, 0};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = T::mfma32(kf[i][ks], qf[ks], s);
+      for (int ks = 0; ks < KS; ++ks) sc[i] = T::mfma32(kf[i][ks], qf[ks], sc[i]);
+    }
+    if (more) load_k(next);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float y = s[r] * a.scale2;
+        float y = sc[i][r] * a.scale2;
         if (a.softcap2 > 0.0f) {  // cap tanh(y / cap), tanh z = 1 - 2 / (e^2z + 1)
           const float e = exp2_(y * a.inv_cap);
           y = a.softcap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f));
         }
-        y = (ok >> (i * 16 + quad * 4 + r)) & 1 ? y : -INFINITY;
+        y = (cur.ok >> (i * 16 + quad * 4 + r)) & 1 ? y : -INFINITY;
         x[i * 4 + r] = y;
         mt = fmaxf(mt, y);
       }
@@ -201,10 +261,10 @@ __global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
       pf[j / 2] = T::pack(p0_, p1_);
     }
     l = fmaf(l, alpha, sum);
-    if (ok != (uint32_t)((1ull << TP) - 1)) {  // what stands in other rows may be anything
+    if (cur.ok != FULL) {  // what stands in other rows may be anything
 #pragma unroll
       for (int j = 0; j < NP; ++j)
-        if (!((ok >> ((j >> 2) * 16 + quad * 4 + (j & 3))) & 1))
+        if (!((cur.ok >> ((j >> 2) * 16 + quad * 4 + (j & 3))) & 1))
 #pragma unroll
           for (int i = 0; i < CG; ++i)
 #pragma unroll
@@ -226,6 +286,9 @@ __global__ __launch_bounds__(NW * 64) void k_paged_attn(PagedAttnArgs a) {
           acc = T::mfma16(v2u{vt[0], vt[1]}, v2u{pf[0], pf[1]}, acc);
         o[i][c] = acc;
       }
+    if (more) load_v(next);
+    cur = next;
+    if (t + 2 * NW < rg.t1) next = find(t + 2 * NW);
   }
   l = quad_sum(l);
 
@@ -311,23 +374,32 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a) {
   if (a.lse && col == 0) a.lse[row] = L != 0.0f ? (M + __builtin_amdgcn_logf(L) - T::kWeightBits) * kLn2 : -INFINITY;
 }
 
-template <typename T, int HD>
-hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
-  constexpr int NW = 4, TP = tile_positions<HD>();
-  // a window that does not start on a tile reaches into one more
-  const int tiles = (max_len + TP - 1) / TP + (a.window > 0 ? 1 : 0);
-  a.chunk_tiles = std::max(1, (tiles + a.s_max - 1) / a.s_max);
+template <typename T, int HD, bool SMALL>
+hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t st) {
+  constexpr int NW = 4;
   const int G = std::min(16, a.gqa);
   const int64_t blocks = (int64_t)a.num_seqs * a.num_kv * a.head_groups * a.s_max;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const size_t lds = ((size_t)NW * G * (HD + 8) + 2 * NW * 16) * sizeof(float);
   if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_attn<T, HD, NW>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const hipError_t e =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_attn<T, HD, NW, SMALL>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  k_paged_attn<T, HD, NW><<<(int)blocks, NW * 64, lds, st>>>(a);
-  hipError_t e = hipGetLastError();
+  k_paged_attn<T, HD, NW, SMALL><<<(int)blocks, NW * 64, lds, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int HD>
+hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
+  constexpr int TP = tile_positions<HD>();
+  // a window that does not start on a tile reaches into one more
+  const int len = a.window > 0 ? std::min(a.window, max_len) : max_len;
+  const int64_t tiles = ((int64_t)len + TP - 1) / TP + (a.window > 0 ? 1 : 0);
+  a.chunk_tiles = (int)std::max<int64_t>(1, (tiles + a.s_max - 1) / a.s_max);
+  const hipError_t e =
+      a.page_shift < 4 ? launch_attn<T, HD, true>(a, st) : launch_attn<T, HD, false>(a, st);
   if (e != hipSuccess || a.s_max == 1) return e;
   const int rpb = 256 / (HD / 4);
   const int64_t rows = (int64_t)a.num_seqs * a.num_q;
@@ -350,7 +422,7 @@ hipError_t launch_hd(const PagedAttnArgs& a, int hd, int max_len, hipStream_t st
 // Workgroups of 4 waves, a tile a wave at a time: enough splits for `target`
 // workgroups, none of fewer than four tiles.
 int paged_attn_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len, int window) {
-  const int tp = head_dim == 512 ? 16 : 32;
+  const int tp = head_dim >= 256 ? 16 : 32;
   int64_t len = window > 0 ? std::min(max_kv_len, window) : max_kv_len;
   const int64_t tiles = (len + tp - 1) / tp + (window > 0 ? 1 : 0);
   const int64_t groups = (int64_t)num_seqs * num_kv * ((num_q / num_kv + 15) / 16);
