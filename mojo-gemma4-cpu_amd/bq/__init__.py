@@ -791,10 +791,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 def _half(*tensors):
     """The BQ_DT_* of 16-bit device tensors of one type."""
     dt = tensors[0].dtype
-    if dt not in (torch.bfloat16, torch.float16):
+    if dt is not torch.bfloat16 and dt is not torch.float16:
         raise TypeError(f"expected bfloat16 or float16, got {dt}")
     for t in tensors:
-        if t is not None and t.dtype != dt:
+        if t is not None and t.dtype is not dt:
             raise TypeError(f"expected {dt} throughout, got {t.dtype}")
     return _DTYPES[dt]
 
@@ -815,24 +815,29 @@ def _ptr(t):
 
 
 def _rows(t: torch.Tensor, width: int):
-    """The row stride of a [rows, width] tensor whose rows are contiguous."""
-    if t.dim() != 2 or t.shape[1] != width:
-        raise ValueError(f"expected [rows, {width}], got {tuple(t.shape)}")
-    if width > 1 and t.stride(1) != 1:
+    """(rows, row stride) of a [rows, width] tensor whose rows are contiguous."""
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise ValueError(f"expected [rows, {width}], got {tuple(shape)}")
+    n = shape[0]
+    row, value = t.stride()
+    if value != 1 and width > 1:
         raise ValueError("libbq takes rows of contiguous values")
-    return t.stride(0) if t.shape[0] > 1 else width
+    return n, row if n > 1 else width
 
 
 def _table(base_rows: torch.Tensor):
-    _dev(base_rows, torch.int32)
-    if base_rows.dim() != 2:
-        raise ValueError("base_rows: int32 [sequences, pages]")
-    return base_rows.shape
+    shape = base_rows.shape
+    if base_rows.dtype is not torch.int32:
+        raise TypeError(f"base_rows: expected torch.int32, got {base_rows.dtype}")
+    if len(shape) != 2 or not base_rows.is_contiguous():
+        raise ValueError("base_rows: contiguous int32 [sequences, pages]")
+    return shape
 
 
 def _flat(t: torch.Tensor, dtype, n: int, name: str):
     """A contiguous tensor of n values (its device is _here's to check)."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name}: expected {n} contiguous values, got {tuple(t.shape)}")
@@ -889,28 +894,28 @@ def rope_append(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, num_q
     pair_stride None: rope_half (pairs by halves), 0: neighbours."""
     dt = _half(q, k, v, k_cache, v_cache, q_norm, k_norm, out)
     st = _here(q, k, v, inv_freq, positions, base_rows, k_cache, v_cache, seq_ids, q_norm, k_norm, out)
-    T, kw = q.shape[0], num_kv * head_dim
-    qs, ks, vs = _rows(q, num_q * head_dim), _rows(k, kw), _rows(v, kw)
-    if k.shape[0] != T or v.shape[0] != T:
-        raise ValueError(f"rope_append: {T} rows of q, {k.shape[0]} of k, {v.shape[0]} of v")
+    qw, kw = num_q * head_dim, num_kv * head_dim
+    (T, qs), (kt, ks), (vt, vs) = _rows(q, qw), _rows(k, kw), _rows(v, kw)
+    if kt != T or vt != T:
+        raise ValueError(f"rope_append: {T} rows of q, {kt} of k, {vt} of v")
     slots = _caches(k_cache, v_cache, kw)
     _flat(positions, torch.int32, T, "positions")
     if seq_ids is not None:
         _flat(seq_ids, torch.int32, T, "seq_ids")
-    for g in (q_norm, k_norm):
-        if g is not None:
-            _flat(g, q.dtype, head_dim, "gain")
+    if q_norm is not None:
+        _flat(q_norm, q.dtype, head_dim, "q_norm")
+    if k_norm is not None:
+        _flat(k_norm, q.dtype, head_dim, "k_norm")
     half = 0 if inv_freq is None else _dev(inv_freq, torch.float32).numel()
     n, width = _table(base_rows)
     if sqrt_n is None or n_eps is None:
         sqrt_n, n_eps = head_dim ** 0.5, head_dim * 1e-6
     if out is None:
-        out = torch.empty((T, num_q * head_dim), dtype=q.dtype, device=q.device)
-        os_ = num_q * head_dim
+        out, os_ = torch.empty((T, qw), dtype=q.dtype, device=q.device), qw
     else:
-        os_ = _rows(out, num_q * head_dim)
-        if out.shape[0] != T:
-            raise ValueError(f"out: expected {T} rows, got {out.shape[0]}")
+        ot, os_ = _rows(out, qw)
+        if ot != T:
+            raise ValueError(f"out: expected {T} rows, got {ot}")
     _check(_lib.bq_rope_append(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, _ptr(q_norm), _ptr(k_norm), int(norm_v),
         sqrt_n, n_eps, _ptr(inv_freq), half, half if pair_stride is None else pair_stride, mscale,
@@ -942,9 +947,8 @@ def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv:
     scale None: head_dim ** -0.5; lse: f32 [S, num_q] to fill."""
     dt = _half(q, k_cache, v_cache, out)
     st = _here(q, k_cache, v_cache, base_rows, kv_lens, workspace, out, lse)
-    S, kw = q.shape[0], num_kv * head_dim
-    qs = _rows(q, num_q * head_dim)
-    slots = _caches(k_cache, v_cache, kw)
+    S, qs = _rows(q, num_q * head_dim)
+    slots = _caches(k_cache, v_cache, num_kv * head_dim)
     n, width = _table(base_rows)
     if n < S:
         raise ValueError(f"base_rows: {n} rows for {S} sequences")
@@ -966,8 +970,11 @@ def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv:
         base_rows.data_ptr(), width, page_shift, kv_lens.data_ptr(), out.data_ptr(), _ptr(lse), S,
         num_q, num_kv, head_dim, window, head_dim ** -0.5 if scale is None else scale, softcap, dt,
         max_kv_len, s_max, _ptr(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), st))
+        0 if workspace is None else workspace.nbytes, st))
     return out
+
+
+_nbytes = torch.Tensor.nbytes.__get__
 
 
 class CacheArrays:
@@ -976,14 +983,17 @@ class CacheArrays:
     cache, or by each call that is given a list."""
 
     def __init__(self, arrays, slots: int):
-        self.arrays, self.slots, table = list(arrays), slots, []
-        for i, a in enumerate(self.arrays):
-            n = a.numel()
-            if a.dim() < 1 or a.shape[0] != slots or n == 0 or not a.is_contiguous():
-                raise ValueError(f"array {i}: expected {slots} contiguous rows, got "
-                                 f"{tuple(a.shape)}")
-            table += (a.data_ptr(), n // slots * a.element_size())
-        self.table = (C.c_int64 * max(len(table), 1))(*table)  # bq_cache_array pairs
+        self.arrays, self.slots = list(arrays), slots
+        n, t = len(self.arrays), torch.Tensor
+        sizes = list(map(_nbytes, self.arrays))
+        if (0 in sizes or not all(map(t.is_contiguous, self.arrays)) or
+                any([a.dim() == 0 or a.shape[0] != slots for a in self.arrays])):
+            raise ValueError(f"arrays: expected {slots} contiguous rows each, got "
+                             f"{[tuple(a.shape) for a in self.arrays]}")
+        self.table = (C.c_int64 * max(2 * n, 1))()  # bq_cache_array pairs
+        self.table[0:2 * n:2] = list(map(t.data_ptr, self.arrays))
+        self.table[1:2 * n:2] = [s // slots for s in sizes]
+        self.device = set(map(t.get_device, self.arrays))
 
 
 def _cache_arrays(arrays, slots: int):
@@ -992,6 +1002,14 @@ def _cache_arrays(arrays, slots: int):
     if arrays.slots != slots:
         raise ValueError(f"arrays have {arrays.slots} rows, the pool {slots}")
     return arrays
+
+
+def _arrays_here(arrays, *tensors):
+    """_here for a cache's arrays too."""
+    st = _here(*tensors)
+    if arrays.device and arrays.device != {tensors[0].get_device()}:
+        raise ValueError(f"libbq launches on the current device; got arrays on {arrays.device}")
+    return st
 
 
 def cache_reorder(arrays, base_rows, lens, refs, parents, page_shift: int, grow=None,
@@ -1008,18 +1026,18 @@ def cache_reorder(arrays, base_rows, lens, refs, parents, page_shift: int, grow=
         _flat(grow, torch.int32, n, "grow")
     pool = _dev(refs, torch.int32).numel()
     arrays = _cache_arrays(arrays, pool << page_shift)
-    st = _here(base_rows, lens, refs, parents, grow, workspace, info, *arrays.arrays)
+    st = _arrays_here(arrays, base_rows, lens, refs, parents, grow, workspace, info)
     if workspace is None:
-        workspace = torch.empty(int(_lib.bq_cache_reorder_workspace_size(n)), dtype=torch.uint8,
+        workspace = torch.empty(_lib.bq_cache_reorder_workspace_size(n), dtype=torch.uint8,
                                 device=base_rows.device)
     if info is None:
         info = torch.empty(4, dtype=torch.int32, device=base_rows.device)
     else:
         _flat(info, torch.int32, 4, "info")
-    _check(_lib.bq_cache_reorder(arrays.table, len(arrays.arrays), base_rows.data_ptr(), lens.data_ptr(),
-                                 refs.data_ptr(), parents.data_ptr(), _ptr(grow), n, width,
-                                 page_shift, pool, info.data_ptr(), workspace.data_ptr(),
-                                 workspace.numel() * workspace.element_size(), st))
+    _check(_lib.bq_cache_reorder(arrays.table, len(arrays.arrays), base_rows.data_ptr(),
+                                 lens.data_ptr(), refs.data_ptr(), parents.data_ptr(), _ptr(grow),
+                                 n, width, page_shift, pool, info.data_ptr(),
+                                 workspace.data_ptr(), workspace.nbytes, st))
     return info
 
 
@@ -1029,17 +1047,17 @@ def cache_compact(arrays, base_rows, refs, page_shift: int, workspace=None, info
     n, width = _table(base_rows)
     pool = _dev(refs, torch.int32).numel()
     arrays = _cache_arrays(arrays, pool << page_shift)
-    st = _here(base_rows, refs, workspace, info, *arrays.arrays)
+    st = _arrays_here(arrays, base_rows, refs, workspace, info)
     if workspace is None:
-        workspace = torch.empty(int(_lib.bq_cache_compact_workspace_size(pool)),
+        workspace = torch.empty(_lib.bq_cache_compact_workspace_size(pool),
                                 dtype=torch.uint8, device=base_rows.device)
     if info is None:
         info = torch.empty(4, dtype=torch.int32, device=base_rows.device)
     else:
         _flat(info, torch.int32, 4, "info")
-    _check(_lib.bq_cache_compact(arrays.table, len(arrays.arrays), base_rows.data_ptr(), refs.data_ptr(), n,
-                                 width, page_shift, pool, info.data_ptr(), workspace.data_ptr(),
-                                 workspace.numel() * workspace.element_size(), st))
+    _check(_lib.bq_cache_compact(arrays.table, len(arrays.arrays), base_rows.data_ptr(),
+                                 refs.data_ptr(), n, width, page_shift, pool, info.data_ptr(),
+                                 workspace.data_ptr(), workspace.nbytes, st))
     return info
 
 
@@ -1059,7 +1077,7 @@ def beam_select(logits, scores, n: int | None = None, finished=None, eos_id: int
     rows, vocab = logits.shape
     if rows != b * k:
         raise ValueError(f"logits: expected {b * k} rows, got {rows}")
-    stride = _rows(logits, vocab)
+    _, stride = _rows(logits, vocab)
     if n is None:
         n = k
     if finished is not None:
@@ -1067,7 +1085,7 @@ def beam_select(logits, scores, n: int | None = None, finished=None, eos_id: int
               "finished")
     d = logits.device
     if workspace is None:
-        workspace = torch.empty(int(_lib.bq_beam_select_workspace_size(rows, vocab)),
+        workspace = torch.empty(_lib.bq_beam_select_workspace_size(rows, vocab),
                                 dtype=torch.uint8, device=d)
     if out is None:
         out = (torch.empty((b, n), dtype=torch.float32, device=d),
@@ -1083,7 +1101,7 @@ def beam_select(logits, scores, n: int | None = None, finished=None, eos_id: int
                                scores.data_ptr(), _ptr(finished), b, k, vocab, n, eos_id,
                                out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
                                out[3].data_ptr() if len(out) > 3 else None, workspace.data_ptr(),
-                               workspace.numel() * workspace.element_size(), st))
+                               workspace.nbytes, st))
     return out
 
 

@@ -3,6 +3,9 @@
 // caller's stream.
 #include <stdarg.h>
 
+#include <atomic>
+#include <chrono>
+
 #include "../../include/bq_api.h"
 #include "bq_kernels.hpp"
 #include "bq_pages.hpp"
@@ -71,6 +74,26 @@ int pool_args(const char* who, const bq_cache_array* arrays, int num_arrays,
 }
 
 }  // namespace
+
+namespace bq {
+
+// A number that no other launch of this process has, and that memory does not hold by
+// chance: a mixed count from a start of the clock's and the address space's choosing.
+uint64_t launch_tag() {
+  static std::atomic<uint64_t> count{
+      (uint64_t)std::chrono::system_clock::now().time_since_epoch().count() * 0xD1342543DE82EF95ull ^
+      reinterpret_cast<uintptr_t>(&launch_tag) << 16};
+  uint64_t x;
+  do {
+    x = count.fetch_add(1, std::memory_order_relaxed) + 0x9E3779B97F4A7C15ull;
+    x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
+    x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
+    x ^= x >> 31;
+  } while (x == 0);
+  return x;
+}
+
+}  // namespace bq
 
 extern "C" {
 
@@ -144,7 +167,7 @@ int bq_paged_attention_splits(int num_seqs, int num_q, int num_kv, int head_dim,
 
 size_t bq_paged_attention_workspace_size(int num_seqs, int num_q, int head_dim, int s_max) {
   if (num_seqs <= 0 || num_q <= 0 || head_dim <= 0 || s_max <= 1) return 0;
-  return (size_t)num_seqs * num_q * s_max * ((size_t)head_dim + 2) * sizeof(float);
+  return (size_t)num_seqs * num_q * s_max * ((size_t)head_dim + 4) * sizeof(float);
 }
 
 int bq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,

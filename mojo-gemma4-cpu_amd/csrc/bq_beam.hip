@@ -22,8 +22,9 @@ namespace bq {
 namespace {
 
 constexpr int kPart = 2048;          // logits per part
-constexpr int kPickThreads = 1024;
-constexpr int kListed = 2048;        // candidates ranked in LDS
+constexpr int kPickThreads = 1024, kWaves = kPickThreads / 64;
+constexpr int kListed = 1024;        // candidates ranked in LDS
+constexpr int kFusedParts = 2048;    // parts of a request that one launch does all of
 
 struct BeamPart {
   double sum;  // of e^(x - max)
@@ -124,6 +125,27 @@ struct PartValues {
   __device__ int token(int i, int e) const { return first + (i * 64 + lane_id()) * In::N + e; }
 };
 
+// the maximum of a part and its exponentials' sum, in lane 0
+template <typename In>
+__device__ inline BeamPart sum_part(const PartValues<In>& p, const double* table) {
+  float m = -INFINITY;  // NaN is no candidate and adds nothing
+#pragma unroll
+  for (int i = 0; i < p.WORDS; ++i)
+#pragma unroll
+    for (int e = 0; e < In::N; ++e) m = fmaxf(m, p.x[i][e]);
+  m = wave_all_max(m);
+  double s = 0.0;
+  if (m > -INFINITY && m < INFINITY) {
+    const Exp64 ex(table, m);
+#pragma unroll
+    for (int i = 0; i < p.WORDS; ++i)
+#pragma unroll
+      for (int e = 0; e < In::N; ++e) s = ex(p.x[i][e], s);
+    s = wave_all_sum(s);
+  }
+  return BeamPart{s, m, 0};
+}
+
 template <typename In>
 __global__ __launch_bounds__(256) void k_beam_parts(BeamArgs a) {
   __shared__ double table[32];
@@ -137,24 +159,8 @@ __global__ __launch_bounds__(256) void k_beam_parts(BeamArgs a) {
   exp64_table(table);  // while the logits come
   __syncthreads();
   if (!on) return;
-  float m = -INFINITY;  // NaN is no candidate and adds nothing
-#pragma unroll
-  for (int i = 0; i < p.WORDS; ++i)
-#pragma unroll
-    for (int e = 0; e < In::N; ++e) m = fmaxf(m, p.x[i][e]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-  double s = 0.0;
-  if (m > -INFINITY && m < INFINITY) {
-    const Exp64 ex(table, m);
-#pragma unroll
-    for (int i = 0; i < p.WORDS; ++i)
-#pragma unroll
-      for (int e = 0; e < In::N; ++e) s = ex(p.x[i][e], s);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-  }
-  if (lane_id() == 0) static_cast<BeamPart*>(a.workspace)[w] = BeamPart{s, m, 0};
+  const BeamPart part = sum_part(p, table);
+  if (lane_id() == 0) static_cast<BeamPart*>(a.workspace)[w] = part;
 }
 
 // a candidate: a better score first, then a lower place (beam, part or token)
@@ -170,12 +176,15 @@ constexpr Cand kNone{-INFINITY, kNowhere};
 
 struct PickLds {
   double table[32];
-  Cand group[64];               // the best of each group of threads
+  BeamPart parts[kFusedParts];  // FUSED: the request's
+  Cand group[kWaves];           // the best of each wave
+  float top[64];                // of each 16 threads
+  int rank[64];
   Cand list[kListed];
   double lse[kMaxBeams], score[kMaxBeams];
   Cand chosen[kMaxPicks];
-  Cand bound;
-  int part[kMaxPicks];
+  double bound;
+  int64_t part[kMaxPicks];
   int count;
 };
 
@@ -208,12 +217,20 @@ __device__ inline int pick(PickLds& s, int n, Cand bound, Each&& each) {
   __syncthreads();
   const int m = s.count;
   if (m <= kListed) {
-    for (int i = threadIdx.x; i < m; i += kPickThreads) {
-      const Cand c = s.list[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < m; ++j) rank += before(s.list[j], c);
-      if (rank < n) s.chosen[rank] = c;
+    // 64 candidates at a time, 16 threads each
+    for (int i0 = 0; i0 < m; i0 += 64) {
+      const int i = i0 + (threadIdx.x & 63);
+      if (threadIdx.x < 64) s.rank[threadIdx.x] = 0;
+      __syncthreads();
+      if (i < m) {
+        const Cand c = s.list[i];
+        int rank = 0;
+        for (int j = threadIdx.x >> 6; j < m; j += kWaves) rank += before(s.list[j], c);
+        if (rank) atomicAdd(&s.rank[threadIdx.x & 63], rank);
+      }
+      __syncthreads();
+      if (threadIdx.x < 64 && i < m && s.rank[threadIdx.x] < n)
+        s.chosen[s.rank[threadIdx.x]] = s.list[i];
     }
     __syncthreads();
     return min(n, m);
@@ -229,7 +246,7 @@ __device__ inline int pick(PickLds& s, int n, Cand bound, Each&& each) {
     if (lane_id() == 0) s.group[threadIdx.x >> 6] = best;
     __syncthreads();
     best = s.group[0];
-    for (int w = 1; w < kPickThreads / 64; ++w)
+    for (int w = 1; w < kWaves; ++w)
       if (before(s.group[w], best)) best = s.group[w];
     if (threadIdx.x == 0) s.chosen[r] = best;
     __syncthreads();
@@ -239,29 +256,57 @@ __device__ inline int pick(PickLds& s, int n, Cand bound, Each&& each) {
   return r;
 }
 
-template <typename In>
+// FUSED: the parts too, one a wave; the request's last workgroup picks.
+template <typename In, bool FUSED>
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
   __shared__ PickLds s;
-  const int b = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int total = a.beams * a.parts, blocks = (total + kWaves - 1) / kWaves;
+  const int b = FUSED ? blockIdx.x / blocks : blockIdx.x;
   const int64_t row0 = (int64_t)b * a.beams;
-  const BeamPart* parts = static_cast<const BeamPart*>(a.workspace) + row0 * a.parts;
-  exp64_table(s.table);
+  BeamPart* parts = static_cast<BeamPart*>(a.workspace) + row0 * a.parts;
+  if constexpr (FUSED) {
+    const int place = blockIdx.x - b * blocks, id = place * kWaves + wave, k = id / a.parts;
+    const bool on = id < total && !(a.finished && a.finished[row0 + k]);
+    PartValues<In> p;
+    if (on)
+      p.load(static_cast<const typename In::raw*>(a.logits) + (row0 + k) * a.row_stride, a.vocab,
+             id - k * a.parts);
+    exp64_table(s.table);  // while the logits come
+    __syncthreads();
+    if (on) {
+      const BeamPart part = sum_part(p, s.table);
+      if (lane == 0) {
+        uint64_t* w = reinterpret_cast<uint64_t*>(parts + id);
+        store_agent(w, __builtin_bit_cast(uint64_t, part.sum));
+        store_agent(w + 1, __float_as_uint(part.max));
+      }
+    }
+    stores_done();
+    if (!last_of(a.marks + (int64_t)b * blocks, 1, blocks, place, a.tag, &s.count)) return;
+    for (int i = threadIdx.x; i < total; i += kPickThreads) {
+      const uint64_t* w = reinterpret_cast<const uint64_t*>(parts + i);
+      const uint64_t sum = load_agent(w), max = load_agent(w + 1);
+      s.parts[i] = BeamPart{__builtin_bit_cast(double, sum), __uint_as_float((uint32_t)max), 0};
+    }
+    parts = s.parts;
+  } else {
+    exp64_table(s.table);
+  }
   __syncthreads();
 
-  for (int k = wave; k < a.beams; k += kPickThreads / 64) {
+  for (int k = wave; k < a.beams; k += kWaves) {
     double lse = 0.0;
     if (!(a.finished && a.finished[row0 + k])) {
       const BeamPart* p = parts + (int64_t)k * a.parts;
       float m = -INFINITY;
       for (int i = lane; i < a.parts; i += 64) m = fmaxf(m, p[i].max);
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+      m = wave_all_max(m);
       const Exp64 ex(s.table, m);
       double sum = 0.0;
       for (int i = lane; i < a.parts; i += 64)
         if (p[i].max > -INFINITY) sum = __builtin_fma(p[i].sum, ex(p[i].max, 0.0), sum);
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+      sum = wave_all_sum(sum);
       lse = m < INFINITY ? (double)m + log(sum) : NAN;  // a row with +inf has no candidates
     }
     if (lane == 0) {
@@ -271,68 +316,71 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
   }
   __syncthreads();
 
-  // the n parts with the best maxima
-  const int total = a.beams * a.parts;
+  // the n parts with the best maxima; a place is (beam, part) and then (beam, token)
+  const int chunks = (a.parts + 63) / 64;
   auto each_part = [&](auto&& f) {
-    for (int id = threadIdx.x; id < total; id += kPickThreads) {
-      const int k = id / a.parts;
-      Cand c{-INFINITY, id};
+    for (int i = wave; i < a.beams * chunks; i += kWaves) {
+      const int k = i / chunks, part = (i - k * chunks) * 64 + lane;
+      if (part >= a.parts) continue;
+      Cand c{-INFINITY, (int64_t)k << 32 | part};
       if (a.finished && a.finished[row0 + k]) {
-        if (id == k * a.parts) c.score = s.score[k];
+        if (part == 0) c.score = s.score[k];
       } else {
-        const float m = parts[id].max;
+        const float m = parts[k * a.parts + part].max;
         if (m > -INFINITY) c.score = s.score[k] + ((double)m - s.lse[k]);
       }
       if (c.score > -INFINITY) f(c);
     }
   };
-  // What is worse than the n-th best of all groups' best is not among the n best.
-  constexpr int lanes = 16, groups = kPickThreads / lanes;
-  Cand best = kNone;
-  each_part([&](const Cand& c) {
-    if (before(c, best)) best = c;
-  });
-  best = lanes_best<lanes>(best);
-  if (lane % lanes == 0) s.group[threadIdx.x / lanes] = best;
+  // The n-th best of the best scores of every 16 threads, rounded down to 32 bits: n
+  // parts are no worse, and what is worse is not among the n best.
+  float top = -INFINITY;
+  each_part([&](const Cand& c) { top = fmaxf(top, __double2float_rd(c.score)); });
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane % 16 == 0) s.top[threadIdx.x / 16] = top;
   __syncthreads();
-  best = s.group[lane];
-  int rank = 0;
-#pragma unroll 8
-  for (int g = 0; g < groups; ++g) rank += before(s.group[g], best);
-  if (wave == 0 && best.at != kNowhere && rank == a.n - 1) s.bound = best;
-  const bool enough = __popcll(__ballot(best.at != kNowhere)) >= a.n;
+  if (wave == 0) {
+    const int w = __float_as_int(s.top[lane]);
+    const uint32_t key = w < 0 ? ~(uint32_t)w : (uint32_t)w | 0x80000000u;  // in the floats' order
+    uint32_t nth = 0;  // the largest that n keys reach, from its first bit on
+    for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+      if (__popcll(__ballot(key >= (nth | bit))) >= a.n) nth |= bit;
+    if (lane == 0) s.bound = __uint_as_float(nth & 0x80000000u ? nth & 0x7FFFFFFFu : ~nth);
+  }
   __syncthreads();
-  Cand bound = enough ? s.bound : kNone;
+  Cand bound{s.bound, kNowhere - 1};
   const int picks = pick(s, a.n, bound, each_part);
 
   // the n best of their elements: no worse than the worst part's best
-  for (int q = threadIdx.x; q < picks; q += kPickThreads) s.part[q] = (int)s.chosen[q].at;
-  bound = picks < a.n ? kNone : Cand{s.chosen[picks - 1].score, kNowhere - 1};
+  for (int q = threadIdx.x; q < picks; q += kPickThreads) s.part[q] = s.chosen[q].at;
+  bound.score = picks < a.n ? -INFINITY : s.chosen[picks - 1].score;
   __syncthreads();
   auto each_value = [&](auto&& f) {
 #pragma unroll 1
-    for (int q = wave; q < picks; q += kPickThreads / 64) {
-      const int id = s.part[q], k = id / a.parts, part = id - k * a.parts;
+    for (int q = wave; q < picks; q += kWaves) {
+      const int k = (int)(s.part[q] >> 32), part = (int)s.part[q];
       const double sc = s.score[k], lse = s.lse[k];
       if (a.finished && a.finished[row0 + k]) {
-        if (lane == 0) f(Cand{sc, (int64_t)k * a.vocab + a.eos_id});
+        if (lane == 0) f(Cand{sc, (int64_t)k << 32 | a.eos_id});
         continue;
       }
       const typename In::raw* row =
           static_cast<const typename In::raw*>(a.logits) + (row0 + k) * a.row_stride;
       PartValues<In> p;
       p.load(row, a.vocab, part);
-      uint32_t good = 0;  // few pass: they are read once more
+      // what may pass, by a bound in 32 bits from below; those few are read once more
+      const float least = __double2float_rd(bound.score - sc + lse - 1e-9);
+      uint32_t good = 0;
 #pragma unroll
       for (int i = 0; i < p.WORDS; ++i)
 #pragma unroll
-        for (int e = 0; e < In::N; ++e) {
-          const double v = sc + ((double)p.x[i][e] - lse);
-          good |= (uint32_t)(v >= bound.score && v > -INFINITY) << (i * In::N + e);
-        }
+        for (int e = 0; e < In::N; ++e) good |= (uint32_t)(p.x[i][e] >= least) << (i * In::N + e);
       for (; good; good &= good - 1) {
         const int at = __builtin_ctz(good), v = p.token(at / In::N, at % In::N);
-        f(Cand{sc + ((double)In::value(row[v]) - lse), (int64_t)k * a.vocab + v});
+        const double score =
+            v >= 0 && v < a.vocab ? sc + ((double)In::value(row[v]) - lse) : -INFINITY;
+        if (score >= bound.score && score > -INFINITY) f(Cand{score, (int64_t)k << 32 | v});
       }
     }
   };
@@ -341,8 +389,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
     const int64_t o = (int64_t)b * a.n + r;
     const bool any = r < found;
     const Cand c = any ? s.chosen[r] : kNone;
-    const int k = any ? (int)(c.at / a.vocab) : -1;
-    const int v = any ? (int)(c.at - (int64_t)k * a.vocab) : -1;
+    const int k = any ? (int)(c.at >> 32) : -1, v = any ? (int)c.at : -1;
     a.out_scores[o] = any ? (float)c.score : -INFINITY;
     a.out_parents[o] = any ? (int)(row0 + k) : -1;
     a.out_tokens[o] = v;
@@ -352,13 +399,22 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
 }
 
 template <typename In>
-hipError_t launch(const BeamArgs& a, hipStream_t st) {
-  const int64_t waves = (int64_t)a.batch * a.beams * a.parts;
-  if ((waves + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
-  k_beam_parts<In><<<(int)((waves + 3) / 4), 256, 0, st>>>(a);
+hipError_t launch(BeamArgs a, hipStream_t st) {
+  const int64_t total = (int64_t)a.beams * a.parts, blocks = (total + kWaves - 1) / kWaves;
+  // One launch while all of its workgroups run at once (4 beams of 262144 tokens); more
+  // stream better as small ones of their own.
+  if (total <= kFusedParts && a.batch * blocks <= tune().cus) {
+    a.tag = launch_tag();
+    a.marks = reinterpret_cast<uint64_t*>(static_cast<BeamPart*>(a.workspace) + a.batch * total);
+    if (a.batch * blocks > INT32_MAX) return hipErrorInvalidValue;
+    k_beam_pick<In, true><<<(int)(a.batch * blocks), kPickThreads, 0, st>>>(a);
+    return hipGetLastError();
+  }
+  if ((a.batch * total + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
+  k_beam_parts<In><<<(int)((a.batch * total + 3) / 4), 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  k_beam_pick<In><<<a.batch, kPickThreads, 0, st>>>(a);
+  k_beam_pick<In, false><<<a.batch, kPickThreads, 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -366,8 +422,9 @@ hipError_t launch(const BeamArgs& a, hipStream_t st) {
 
 // rows that start off a 16-byte boundary have up to 7 values ahead of their first
 int beam_parts(int vocab) { return (vocab + 7 + kPart - 1) / kPart; }
+// the parts, and a mark for each workgroup (there are no more of them than parts)
 size_t beam_workspace(int64_t rows, int vocab) {
-  return (size_t)rows * beam_parts(vocab) * sizeof(BeamPart);
+  return (size_t)rows * beam_parts(vocab) * (sizeof(BeamPart) + sizeof(uint64_t));
 }
 
 hipError_t launch_beam_select(const BeamArgs& a, int dtype_bytes, bool f16, hipStream_t st) {

@@ -27,8 +27,10 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kTableThreads = 512;
+constexpr int kBatch = 8;           // loads of a thread that are on their way at once
+constexpr int kOwned = 2048;        // wanted pages whose sequences k_reorder_plan lists
 constexpr int kTileEntries = 1024;  // table entries of a k_reorder_tables workgroup
-constexpr int64_t kOneBytes = 56000;  // tables and counts that k_reorder_plan<true> keeps in LDS
+constexpr int64_t kOneBytes = 52000;  // tables and counts that k_reorder_plan<true> keeps in LDS
 
 struct CopyItem {
   int32_t src, dst, rows, pad;
@@ -94,10 +96,18 @@ __device__ inline void count_children(const ReorderArgs& a, SeqLds* seq, int thr
 // columns [j0, j0 + width) of the tables: old page numbers to LDS ...
 __device__ inline void load_tile(const ReorderArgs& a, int32_t* tile, int j0, int width,
                                  int threads) {
-  for (int e = threadIdx.x; e < a.num_seqs * width; e += threads) {
-    const int s = e / width;
-    tile[e] = page_number(a.base_rows[(int64_t)s * a.max_pages + j0 + (e - s * width)], a.page_shift,
-                          a.num_pages);
+  const int n = a.num_seqs * width;
+  for (int e0 = threadIdx.x; e0 < n; e0 += kBatch * threads) {
+    int32_t base[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int e = e0 + u * threads, s = e / width;
+      base[u] = e < n ? a.base_rows[(int64_t)s * a.max_pages + j0 + (e - s * width)] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (e0 + u * threads < n)
+        tile[e0 + u * threads] = page_number(base[u], a.page_shift, a.num_pages);
   }
 }
 
@@ -142,6 +152,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
   __shared__ int wsum[kPlanThreads / 64];
   __shared__ __align__(16) int32_t last[kMaxCacheSeqs];
   __shared__ int32_t offset[kMaxCacheSeqs + 1];
+  __shared__ int16_t owner[kOwned];
   __shared__ int ncopy;
   CopyList* list = static_cast<CopyList*>(a.workspace);
   const int n = a.num_seqs, i = threadIdx.x;
@@ -149,7 +160,17 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
   load_seqs(a, seq, kPlanThreads);
   if constexpr (ONE) {
     load_tile(a, tile, 0, a.max_pages, kPlanThreads);
-    for (int q = i; q < pages4; q += kPlanThreads) refs[q] = q < a.num_pages ? a.refs[q] : -1;
+    for (int q0 = i; q0 < pages4; q0 += kBatch * kPlanThreads) {
+      int32_t r[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int q = q0 + u * kPlanThreads;
+        r[u] = q < a.num_pages ? a.refs[q] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (q0 + u * kPlanThreads < pages4) refs[q0 + u * kPlanThreads] = r[u];
+    }
     __syncthreads();
     count_children(a, seq, kPlanThreads);
     __syncthreads();
@@ -173,6 +194,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
   bool leaves = false;
   if (page >= 0) {
     int earlier = 0;
+#pragma unroll 4
     for (int k = 0; k < (i & ~3); k += 4) {
       const v4i l = *reinterpret_cast<const v4i*>(last + k);
 #pragma unroll
@@ -187,16 +209,23 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
   const int incl = block_scan(fresh, wsum, &total);
   if (i < n) offset[i] = incl - fresh;
   if (i == 0) offset[n] = total;
+  if (total <= kOwned)
+    for (int k = incl - fresh; k < incl; ++k) owner[k] = (int16_t)i;
   if (leaves) atomicAdd(&refs[page], -1);  // it stays above 0: the last one keeps it
   __syncthreads();
 
-  // the k-th page that is wanted: a sequence's, found by bisection of the offsets
+  // the k-th page that is wanted: a sequence's, from a list or (many pages for a few
+  // sequences) by bisection of the offsets
   auto give = [&](int k, int page_) {
-    int lo = 0, hi = n - 1;  // the last sequence with offset <= k
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (offset[mid] <= k) lo = mid;
-      else hi = mid - 1;
+    int lo = 0;
+    if (total <= kOwned) {
+      lo = owner[k];
+    } else {
+      for (int hi = n - 1; lo < hi;) {  // the last sequence with offset <= k
+        const int mid = (lo + hi + 1) >> 1;
+        if (offset[mid] <= k) lo = mid;
+        else hi = mid - 1;
+      }
     }
     const SeqPlan s = plan_of(seq[lo]);
     const int j = s.end - (offset[lo + 1] - k);
@@ -292,12 +321,18 @@ __global__ __launch_bounds__(kPlanThreads) void k_compact_plan(CompactArgs a) {
 }
 
 // Rows of pages in every array: a work item is kSegment bytes of one copy of one
-// array, eight 16-byte loads a thread ahead of its stores.
+// array, four 16-byte loads a thread ahead of its stores, which go past the caches (127
+// MB in copies of 0 to 256 KiB: 54 us, 4.7 TB/s; through them 60).  Items are ordered by
+// segment first, then by array: the missing ones of short copies and the small ones of
+// narrow arrays come one after the other, and no workgroup gets more of them than another
+// (66 us the other way round).  More workgroups than run at once
+// gain 1 us there, and cost a call without copies 1.5.
 constexpr int64_t kSegment = 32768;
+constexpr int kCopyBlocks = 2048;
 
 template <typename W>
 __device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
-  constexpr int U = 8;
+  constexpr int U = 4;
   const int n = (int)(bytes / (int64_t)sizeof(W));
   W* dw = reinterpret_cast<W*>(d);
   const W* sw = reinterpret_cast<const W*>(s);
@@ -308,7 +343,7 @@ __device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
       if (k + u * 256 < n) w[u] = sw[k + u * 256];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (k + u * 256 < n) dw[k + u * 256] = w[u];
+      if (k + u * 256 < n) __builtin_nontemporal_store(w[u], dw + k + u * 256);
   }
 }
 
@@ -326,14 +361,15 @@ __global__ __launch_bounds__(256) void k_cache_copy(CacheArrays arrays, const vo
     if (page >= 0) t.base_rows[e] = to[page] << t.page_shift;
     return;
   }
-  const int64_t per = (int64_t)arrays.n * segments, total = (int64_t)list->count * per;
+  const int copies = list->count;
+  const int64_t pairs = (int64_t)copies * arrays.n, total = pairs * segments;
   for (int64_t w = blockIdx.x - table_blocks; w < total; w += gridDim.x - table_blocks) {
-    const int64_t which = w / per;
-    const CopyItem it = list->item[which];
-    const int r = (int)(w - which * per), array = r / segments;
+    const int segment = (int)(w / pairs), r = (int)(w - segment * pairs);
+    const int array = r / copies;
+    const CopyItem it = list->item[r - array * copies];
     const int64_t row = arrays.row_bytes[array];
     uint8_t* data = static_cast<uint8_t*>(arrays.data[array]);
-    const int64_t at = (int64_t)(r - array * segments) * kSegment, bytes = (int64_t)it.rows * row;
+    const int64_t at = segment * kSegment, bytes = (int64_t)it.rows * row;
     if (at >= bytes) continue;
     const int64_t len = bytes - at < kSegment ? bytes - at : kSegment;
     uint8_t* d = data + it.dst * row + at;
@@ -352,7 +388,7 @@ hipError_t launch_copy(const CacheArrays& arrays, void* workspace, int max_items
   const int64_t segments = std::max<int64_t>(1, (most + kSegment - 1) / kSegment);
   const int64_t entries = t ? (int64_t)t->num_seqs * t->max_pages : 0;
   const int64_t table_blocks = (entries + 255) / 256;
-  const int64_t copies = std::min<int64_t>((int64_t)max_items * arrays.n * segments, 4096);
+  const int64_t copies = std::min<int64_t>((int64_t)max_items * arrays.n * segments, kCopyBlocks);
   if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
   if (copies == 0 && table_blocks == 0) return hipSuccess;
   k_cache_copy<<<(int)(table_blocks + std::max<int64_t>(copies, 1)), 256, 0, st>>>(

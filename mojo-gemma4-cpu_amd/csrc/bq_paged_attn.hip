@@ -49,6 +49,32 @@ __device__ inline float quad_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+constexpr int kMlStride = 4;  // floats of workspace per split beside its sums: m, l, mark
+
+// Parts of one row joined: sums scaled from each part's maximum to the common one.
+template <typename T>
+struct Joined {
+  float ms, M, L = 0.0f;
+  v4f32 acc = {0, 0, 0, 0};
+  __device__ void start(float max) {
+    M = max;
+    ms = max == -INFINITY ? 0.0f : max;
+  }
+  __device__ void add(float m, float l, v4f32 v) {
+    const float f = exp2_(m - ms);
+    L = fmaf(f, l, L);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+  }
+  __device__ void store(const PagedAttnArgs& a, int64_t row, int hd, int col) const {
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // a NaN sum stays
+    const v2u w = {T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+    *reinterpret_cast<v2u*>(a.out + row * hd + col) = w;
+    if (a.lse && col == 0)
+      a.lse[row] = L != 0.0f ? (M + __builtin_amdgcn_logf(L) - T::kWeightBits) * kLn2 : -INFINITY;
+  }
+};
+
 // a sequence's positions and the tiles of them that split `split` takes
 struct Range {
   int len, start;  // positions [start, len)
@@ -80,6 +106,14 @@ constexpr int tile_positions() {
   return HD >= 256 ? 16 : 32;
 }
 
+// HD = 256 keeps its queries in LDS, which makes room for three waves (8 sequences of
+// 8000 positions, 8 kv heads: 125 -> 93 us); HD = 512 has one wave either way, which
+// would wait for them (16 x 4096 positions, 2 kv heads: 52 -> 60 us).
+template <int HD>
+constexpr bool queries_in_lds() {
+  return HD == 256;
+}
+
 // Pages of fewer than 16 rows (SMALL) are looked up position by position and their
 // slots passed between lanes; larger ones once per 16 positions, with the wave's
 // address in scalar registers and the lanes' offsets the same for every tile.
@@ -98,16 +132,22 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
   constexpr int NP = TP / 4;             // positions per lane of the value product
   constexpr int LD = HD + 8;             // LDS row: 16 heads 32 bytes apart in the banks
   constexpr uint32_t FULL = (uint32_t)((1ull << TP) - 1);
+  constexpr bool QLDS = queries_in_lds<HD>();
 
-  extern __shared__ float smem[];  // acc [NW][G][LD], then m, l [NW][16] each
+  extern __shared__ float smem[];  // QLDS: queries; acc [NW][G][LD], m, l [NW][16] each; a flag
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, quad = lane >> 4;
 
-  int b = blockIdx.x;
+  // Workgroups go to the 8 dies in turn: those on the same rows (the groups of 16 query
+  // heads of a kv head) are 8 apart, on one die and its cache.
+  int b = blockIdx.x, hg = 0;
+  if (a.head_groups > 1) {
+    hg = b / 8 % a.head_groups;
+    b = b / (8 * a.head_groups) * 8 + b % 8;
+    if (b >= a.num_seqs * a.num_kv * a.s_max) return;
+  }
   const int split = b % a.s_max;
   b /= a.s_max;
-  const int hg = b % a.head_groups;
-  b /= a.head_groups;
   const int kvh = b % a.num_kv, seq = b / a.num_kv;
   const int G = min(16, a.gqa - hg * 16);
   const int head0 = kvh * a.gqa + hg * 16;
@@ -115,13 +155,16 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
   const Range rg = attn_range(a, seq, split, TP);
   if (split > 0 && split >= rg.splits) return;  // split 0 also writes empty rows
 
+  // the queries: in registers, or (large heads) in LDS for all waves
   v4u qf[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qf[ks] = v4u{0, 0, 0, 0};
-  if (n16 < G) {
+  v4u* qs = reinterpret_cast<v4u*>(smem);  // [KS][64]
+  float* part = smem + (QLDS ? KS * 256 : 0);
+  {
     const uint16_t* q = a.q + (int64_t)seq * a.q_stride + (int64_t)(head0 + n16) * HD + quad * 8;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const v4u*>(q + ks * 32);
+    for (int ks = 0; ks < KS; ++ks)
+      if (!QLDS || ks % NW == wave)
+        qf[ks] = n16 < G ? *reinterpret_cast<const v4u*>(q + ks * 32) : v4u{0, 0, 0, 0};
   }
 
   const int32_t* rows = a.base_rows + (int64_t)seq * a.max_pages;
@@ -221,17 +264,25 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     load_v(cur);
     if (t + NW < rg.t1) next = find(t + NW);
   }
+  if constexpr (QLDS) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      if (ks % NW == wave) qs[ks * 64 + lane] = qf[ks];
+    __syncthreads();
+  }
   for (; t < rg.t1; t += NW) {
     const bool more = t + NW < rg.t1;
     // scores in powers of two, -inf where a position takes no part
     float x[NP];
     float mt = -INFINITY;
     v4f32 sc[MT];
+    int here = lane;
+    if constexpr (QLDS) asm volatile("" : "+v"(here));  // read again, not kept in registers
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       sc[i] = v4f32{0, 0, 0, 0};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) sc[i] = T::mfma32(kf[i][ks], qf[ks], sc[i]);
+      for (int ks = 0; ks < KS; ++ks) sc[i] = T::mfma32(kf[i][ks], QLDS ? qs[ks * 64 + here] : qf[ks], sc[i]);
     }
     if (more) load_k(next);
 #pragma unroll
@@ -293,9 +344,9 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
   l = quad_sum(l);
 
   // the waves' parts, joined in LDS: o[i][c][r] is column i 16 CPL + (4 quad + r) CPL + c
-  float* sm = smem + (size_t)NW * G * LD;
+  float* sm = part + (size_t)NW * G * LD;
   if (n16 < G) {
-    float* d = smem + ((size_t)wave * G + n16) * LD;
+    float* d = part + ((size_t)wave * G + n16) * LD;
 #pragma unroll
     for (int i = 0; i < CG; ++i)
 #pragma unroll
@@ -310,37 +361,66 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     }
   }
   __syncthreads();
+  const int64_t row0 = (int64_t)seq * a.num_q + head0;
   const bool whole = rg.splits <= 1;
   for (int e = threadIdx.x; e < G * (HD / 4); e += NW * 64) {
     const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
+    Joined<T> j;
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w * 16 + h]);
-    const float Ms = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
-    v4f32 acc = {0, 0, 0, 0};
+    j.start(M);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = exp2_(sm[w * 16 + h] - Ms);
-      L = fmaf(f, sm[NW * 16 + w * 16 + h], L);
-      const v4f32 v = *reinterpret_cast<const v4f32*>(smem + ((size_t)w * G + h) * LD + col);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
-    }
-    const int64_t row = (int64_t)seq * a.num_q + head0 + h;
+    for (int w = 0; w < NW; ++w)
+      j.add(sm[w * 16 + h], sm[NW * 16 + w * 16 + h],
+            *reinterpret_cast<const v4f32*>(part + ((size_t)w * G + h) * LD + col));
     if (whole) {
-      const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // a NaN sum stays
-      v2u w = {T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
-      *reinterpret_cast<v2u*>(a.out + row * HD + col) = w;
-      if (a.lse && col == 0) a.lse[row] = L != 0.0f ? (M + __builtin_amdgcn_logf(L) - T::kWeightBits) * kLn2 : -INFINITY;
+      j.store(a, row0 + h, HD, col);
     } else {
-      *reinterpret_cast<v4f32*>(a.ws_acc + (row * a.s_max + split) * HD + col) = acc;
-      if (col == 0) {
-        float* ml = a.ws_ml + (row * a.s_max + split) * 2;
-        ml[0] = M;
-        ml[1] = L;
-      }
+      const int64_t at = (row0 + h) * a.s_max + split;
+      store_agent(a.ws_acc + at * HD + col, j.acc[0], j.acc[1]);
+      store_agent(a.ws_acc + at * HD + col + 2, j.acc[2], j.acc[3]);
+      if (col == 0) store_agent(a.ws_ml + at * kMlStride, M, j.L);
     }
+  }
+  if (whole || !a.tag) return;
+
+  // the splits are joined by whoever comes last
+  stores_done();
+  uint64_t* marks = reinterpret_cast<uint64_t*>(a.ws_ml + row0 * a.s_max * kMlStride + 2);
+  if (!last_of(marks, kMlStride / 2, rg.splits, split, a.tag,
+               reinterpret_cast<int*>(sm + 2 * NW * 16)))
+    return;
+  // maxima and sums to LDS, over the waves' parts; then eight splits' sums at a time
+  for (int e = threadIdx.x; e < G * rg.splits; e += NW * 64) {
+    const int h = e / rg.splits, i = e - h * rg.splits;
+    const v2f v = load2_agent(a.ws_ml + ((row0 + h) * a.s_max + i) * kMlStride);
+    part[2 * e] = v[0];
+    part[2 * e + 1] = v[1];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < G * (HD / 4); e += NW * 64) {
+    const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
+    const float* ml = part + 2 * h * rg.splits;
+    const float* acc = a.ws_acc + (row0 + h) * a.s_max * HD + col;
+    Joined<T> j;
+    float M = -INFINITY;
+    for (int i = 0; i < rg.splits; ++i) M = fmaxf(M, ml[2 * i]);
+    j.start(M);
+    for (int i0 = 0; i0 < rg.splits; i0 += 8) {
+      v2f lo[8], hi[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < rg.splits) {
+          lo[i] = load2_agent(acc + (int64_t)(i0 + i) * HD);
+          hi[i] = load2_agent(acc + (int64_t)(i0 + i) * HD + 2);
+        }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < rg.splits)
+          j.add(ml[2 * (i0 + i)], ml[2 * (i0 + i) + 1], v4f32{lo[i][0], lo[i][1], hi[i][0], hi[i][1]});
+    }
+    j.store(a, row0 + h, HD, col);
   }
 }
 
@@ -353,34 +433,30 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a) {
   const int seq = (int)(row / a.num_q), col = (threadIdx.x % TPR) * 4;
   const int S = attn_range(a, seq, 0, tile_positions<HD>()).splits;
   if (S <= 1) return;
-  const float* ml = a.ws_ml + row * a.s_max * 2;
+  const float* ml = a.ws_ml + row * a.s_max * kMlStride;
   const float* acc = a.ws_acc + row * a.s_max * HD + col;
+  Joined<T> j;
   float M = -INFINITY;
-  for (int s = 0; s < S; ++s) M = fmaxf(M, ml[2 * s]);
-  const float Ms = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f;
-  v4f32 r = {0, 0, 0, 0};
+  for (int s = 0; s < S; ++s) M = fmaxf(M, ml[s * kMlStride]);
+  j.start(M);
 #pragma unroll 4
-  for (int s = 0; s < S; ++s) {
-    const float f = exp2_(ml[2 * s] - Ms);
-    L = fmaf(f, ml[2 * s + 1], L);
-    const v4f32 v = *reinterpret_cast<const v4f32*>(acc + (int64_t)s * HD);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = fmaf(f, v[i], r[i]);
-  }
-  const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-  v2u w = {T::pack(r[0] * inv, r[1] * inv), T::pack(r[2] * inv, r[3] * inv)};
-  *reinterpret_cast<v2u*>(a.out + row * HD + col) = w;
-  if (a.lse && col == 0) a.lse[row] = L != 0.0f ? (M + __builtin_amdgcn_logf(L) - T::kWeightBits) * kLn2 : -INFINITY;
+  for (int s = 0; s < S; ++s)
+    j.add(ml[s * kMlStride], ml[s * kMlStride + 1],
+          *reinterpret_cast<const v4f32*>(acc + (int64_t)s * HD));
+  j.store(a, row, HD, col);
 }
+
+constexpr int64_t kJoinBytes = 48 << 10;
 
 template <typename T, int HD, bool SMALL>
 hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t st) {
   constexpr int NW = 4;
   const int G = std::min(16, a.gqa);
-  const int64_t blocks = (int64_t)a.num_seqs * a.num_kv * a.head_groups * a.s_max;
+  int64_t blocks = (int64_t)a.num_seqs * a.num_kv * a.s_max;
+  if (a.head_groups > 1) blocks = (blocks + 7) / 8 * 8 * a.head_groups;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  const size_t lds = ((size_t)NW * G * (HD + 8) + 2 * NW * 16) * sizeof(float);
+  const size_t lds = ((size_t)NW * G * (HD + 8) + 2 * NW * 16 + 4 + (queries_in_lds<HD>() ? HD * 8 : 0)) *
+                     sizeof(float);
   if (lds > 65536) {
     const hipError_t e =
         hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_attn<T, HD, NW, SMALL>),
@@ -398,9 +474,13 @@ hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
   const int len = a.window > 0 ? std::min(a.window, max_len) : max_len;
   const int64_t tiles = ((int64_t)len + TP - 1) / TP + (a.window > 0 ? 1 : 0);
   a.chunk_tiles = (int)std::max<int64_t>(1, (tiles + a.s_max - 1) / a.s_max);
+  // Few partial sums are joined by the attention's last workgroup, which one workgroup
+  // reads in less than a launch takes.
+  const bool fused = a.s_max > 1 && (int64_t)a.s_max * std::min(16, a.gqa) * HD * 4 <= kJoinBytes;
+  a.tag = fused ? launch_tag() : 0;
   const hipError_t e =
       a.page_shift < 4 ? launch_attn<T, HD, true>(a, st) : launch_attn<T, HD, false>(a, st);
-  if (e != hipSuccess || a.s_max == 1) return e;
+  if (e != hipSuccess || a.s_max == 1 || fused) return e;
   const int rpb = 256 / (HD / 4);
   const int64_t rows = (int64_t)a.num_seqs * a.num_q;
   k_paged_merge<T, HD><<<(int)((rows + rpb - 1) / rpb), 256, 0, st>>>(a);
@@ -419,16 +499,21 @@ hipError_t launch_hd(const PagedAttnArgs& a, int hd, int max_len, hipStream_t st
 
 }  // namespace
 
-// Workgroups of 4 waves, a tile a wave at a time: enough splits for `target`
-// workgroups, none of fewer than four tiles.
+// A workgroup (4 waves, a tile each at a time) per compute unit reads at the full rate
+// and leaves the fewest sums to join: 8 sequences of 16384 positions, 8 kv heads of 128:
+// 4 splits 104 us, 12 splits 105, 2 splits 137; 16 of 8000 with 32 query heads on one
+// kv head: 8 splits 20, 24 splits 26.  A few more than that run beside each other,
+// except for heads of 512, of which a unit holds one workgroup.  No split has fewer than
+// six tiles, and a sequence of three rounds has one (7 of 333 positions: 6.7, 3 splits
+// 7.2 us).
 int paged_attn_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len, int window) {
   const int tp = head_dim >= 256 ? 16 : 32;
-  int64_t len = window > 0 ? std::min(max_kv_len, window) : max_kv_len;
+  const int64_t len = window > 0 ? std::min(max_kv_len, window) : max_kv_len;
   const int64_t tiles = (len + tp - 1) / tp + (window > 0 ? 1 : 0);
   const int64_t groups = (int64_t)num_seqs * num_kv * ((num_q / num_kv + 15) / 16);
-  const int64_t target = 512;
-  const int64_t s = std::min((target + groups - 1) / groups, (tiles + 3) / 4);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(s, 256));
+  const int64_t cus = tune().cus, s = head_dim == 512 ? cus / groups : (cus + groups - 1) / groups;
+  if (tiles <= 12) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({s, (tiles + 5) / 6, 256}));
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, int max_len, bool f16,

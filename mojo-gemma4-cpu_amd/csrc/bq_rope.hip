@@ -20,16 +20,11 @@ namespace bq {
 
 namespace {
 
-struct RopeHead {
-  const uint16_t* src;
-  uint16_t* dst;        // null: not written
-  const uint16_t* gain;  // null: none
-  bool norm, turn, on;
-};
+constexpr int64_t kFullWaves = 2048;
 
 // A wave takes 64 / LPH heads of one token at a time, head_dim / 8 = LPH lanes
 // a head and 8 values a lane, IT times over, so that the sines of a lane's
-// pairs serve IT heads.
+// pairs serve IT heads and IT rows are on their way at once.
 template <typename T, int LPH, int IT>
 __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
   constexpr int HPW = 64 / LPH, HD = LPH * 8;
@@ -42,17 +37,10 @@ __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
   const int group = __builtin_amdgcn_readfirstlane((int)(work - tok64 * groups));
   const int lane = lane_id(), c = lane % LPH, sub = lane / LPH;
 
-  const int pos = a.positions[tok];
-  const int seq = a.seq_ids ? a.seq_ids[tok] : tok;
-  if (pos < 0 || seq < 0 || seq >= a.num_seqs) return;  // padding
-  const int64_t slot = page_slot(a.base_rows + (int64_t)seq * a.max_pages, a.max_pages,
-                                 a.page_shift, a.num_slots, pos);
-
   // this lane's pairs: values 8c .. 8c + 7 of a head, their partners in chunk pc
-  int pc = c, i0 = 0;
-  float sign = 0.0f;  // partner's sine term: -1 first of a pair, +1 second, 0 passes
+  int pc = c, i0 = 4 * c;
+  float sign = 0.0f;  // of the partner's sine term; 0: these values pass
   if (a.pair_stride == 0) {
-    i0 = 4 * c;
     sign = 8 * c < 2 * a.rope_half ? 1.0f : 0.0f;
   } else if (8 * c < a.rope_half) {
     i0 = 8 * c;
@@ -63,54 +51,52 @@ __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
     pc = c - a.pair_stride / 8;
     sign = 1.0f;
   }
-  float co[8], si[8];
-  if (sign != 0.0f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = a.pair_stride == 0 ? i0 + (e >> 1) : i0 + e;
-      const double turns = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189533577);
-      const float t = (float)(turns - __builtin_rint(turns));
-      co[e] = a.mscale * __builtin_amdgcn_cosf(t);
-      si[e] = a.mscale * __builtin_amdgcn_sinf(t);
-      if (a.pair_stride == 0) si[e] = (e & 1) ? si[e] : -si[e];
-      else si[e] *= sign;
-    }
-  }
 
-  RopeHead h[IT];
   v4u x[IT], y[IT];
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int head = (group * IT + it) * HPW + sub;
-    RopeHead& r = h[it];
-    r.on = head < heads;
-    r.turn = sign != 0.0f;
-    if (head < a.num_q) {
-      r.src = a.q + (int64_t)tok * a.q_stride + (int64_t)head * HD;
-      r.dst = a.q_out + (int64_t)tok * a.q_out_stride + (int64_t)head * HD;
-      r.gain = a.q_norm;
-      r.norm = a.q_norm != nullptr;
-    } else {
-      const bool is_k = head < a.num_q + a.num_kv;
-      const int kv = head - a.num_q - (is_k ? 0 : a.num_kv);
-      r.src = is_k ? a.k + (int64_t)tok * a.k_stride + (int64_t)kv * HD
-                   : a.v + (int64_t)tok * a.v_stride + (int64_t)kv * HD;
-      r.dst = slot < 0 ? nullptr
-                       : (is_k ? a.k_cache : a.v_cache) + (slot * a.num_kv + kv) * (int64_t)HD;
-      r.gain = is_k ? a.k_norm : nullptr;
-      r.norm = is_k ? a.k_norm != nullptr : a.norm_v != 0;
-      r.turn = r.turn && is_k;
-    }
+    const bool is_q = head < a.num_q, is_k = head < a.num_q + a.num_kv;
+    const uint16_t* src =
+        is_q   ? a.q + (int64_t)tok * a.q_stride + (int64_t)head * HD
+        : is_k ? a.k + (int64_t)tok * a.k_stride + (int64_t)(head - a.num_q) * HD
+               : a.v + (int64_t)tok * a.v_stride + (int64_t)(head - a.num_q - a.num_kv) * HD;
     x[it] = y[it] = v4u{0, 0, 0, 0};
-    if (r.on) {
-      x[it] = *reinterpret_cast<const v4u*>(r.src + 8 * c);
-      y[it] = x[it];
-      if (r.turn && pc != c) y[it] = *reinterpret_cast<const v4u*>(r.src + 8 * pc);
+    if (head < heads) {
+      x[it] = *reinterpret_cast<const v4u*>(src + 8 * c);
+      if (pc != c && is_k) y[it] = *reinterpret_cast<const v4u*>(src + 8 * pc);
     }
   }
+
+  const int pos = a.positions[tok];
+  const int seq = a.seq_ids ? a.seq_ids[tok] : tok;
+  if (pos < 0 || seq < 0 || seq >= a.num_seqs) return;  // padding
+  const int64_t slot = page_slot(a.base_rows + (int64_t)seq * a.max_pages, a.max_pages,
+                                 a.page_shift, a.num_slots, pos);
+  float co[8], si[8];
+  if (sign != 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (a.pair_stride == 0 && (e & 1)) {  // the pair of the value before
+        co[e] = co[e - 1];
+        si[e] = -si[e - 1];
+        continue;
+      }
+      const int i = a.pair_stride == 0 ? i0 + e / 2 : i0 + e;
+      const double turns = (double)pos * ((double)a.inv_freq[i] * 0.15915494309189533577);
+      const float t = (float)(turns - __builtin_rint(turns));
+      co[e] = a.mscale * __builtin_amdgcn_cosf(t);
+      si[e] = a.mscale * __builtin_amdgcn_sinf(t) * (a.pair_stride == 0 ? -1.0f : sign);
+    }
+  }
+
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
-    const RopeHead& r = h[it];
+    const int head = (group * IT + it) * HPW + sub;
+    const bool is_q = head < a.num_q, is_k = !is_q && head < a.num_q + a.num_kv;
+    const uint16_t* gain = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+    const bool norm = is_q || is_k ? gain != nullptr : a.norm_v != 0;
+    const bool turn = sign != 0.0f && (is_q || is_k);
     float v[8], w[8];
     unpack8<T>(x[it], v);
     unpack8<T>(y[it], w);
@@ -119,46 +105,51 @@ __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
     for (int e = 0; e < 8; ++e) ssq = fmaf(v[e], v[e], ssq);
 #pragma unroll
     for (int d = 1; d < LPH; d <<= 1) ssq += __shfl_xor(ssq, d);
-    if (!r.on || !r.dst) continue;
-    if (r.norm) {
+    if (head >= heads || (!is_q && slot < 0)) continue;
+    if (norm) {
       const float inv = a.sqrt_n / __builtin_sqrtf(ssq + a.n_eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= inv, w[e] *= inv;
-      if (r.gain) {
+      if (gain) {
         float g[8], gp[8];
-        unpack8<T>(*reinterpret_cast<const v4u*>(r.gain + 8 * c), g);
-        unpack8<T>(*reinterpret_cast<const v4u*>(r.gain + 8 * pc), gp);
+        unpack8<T>(*reinterpret_cast<const v4u*>(gain + 8 * c), g);
+        unpack8<T>(*reinterpret_cast<const v4u*>(gain + 8 * pc), gp);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= g[e], w[e] *= gp[e];
       }
     }
-    v4u out;
-    if (r.turn) {
+    v4u out = x[it];
+    if (turn) {
       float o[8];
-      if (a.pair_stride == 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e ^ 1], si[e], v[e] * co[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(w[e], si[e], v[e] * co[e]);
-      }
+      for (int e = 0; e < 8; ++e)
+        o[e] = fmaf(a.pair_stride == 0 ? v[e ^ 1] : w[e], si[e], v[e] * co[e]);
       out = pack8<T>(o);
-    } else {
-      out = r.norm ? pack8<T>(v) : x[it];
+    } else if (norm) {
+      out = pack8<T>(v);
     }
-    *reinterpret_cast<v4u*>(r.dst + 8 * c) = out;
+    uint16_t* dst =
+        is_q ? a.q_out + (int64_t)tok * a.q_out_stride + (int64_t)head * HD
+             : (is_k ? a.k_cache : a.v_cache) +
+                   (slot * a.num_kv + (head - a.num_q - (is_k ? 0 : a.num_kv))) * (int64_t)HD;
+    *reinterpret_cast<v4u*>(dst + 8 * c) = out;
   }
 }
 
+template <typename T, int LPH, int IT>
+hipError_t launch_it(const RopeArgs& a, hipStream_t st) {
+  const int per = 64 / LPH * IT, heads = a.num_q + 2 * a.num_kv;
+  const int64_t blocks = ((int64_t)a.num_tokens * ((heads + per - 1) / per) + 3) / 4;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  k_rope_append<T, LPH, IT><<<(int)blocks, 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+// Four times the heads per wave once that still leaves kFullWaves waves.
 template <typename T, int LPH>
 hipError_t launch(const RopeArgs& a, hipStream_t st) {
-  constexpr int HPW = 64 / LPH;
-  const int heads = a.num_q + 2 * a.num_kv;
-  const int64_t waves = (int64_t)a.num_tokens * ((heads + HPW - 1) / HPW);
-  const int64_t blocks = (waves + 3) / 4;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  k_rope_append<T, LPH, 1><<<(int)blocks, 256, 0, st>>>(a);
-  return hipGetLastError();
+  const int64_t lanes = (int64_t)a.num_tokens * (a.num_q + 2 * a.num_kv) * LPH;
+  return lanes >= kFullWaves * 64 * 4 ? launch_it<T, LPH, 4>(a, st) : launch_it<T, LPH, 1>(a, st);
 }
 
 template <typename T>

@@ -63,14 +63,14 @@ def test_attention_refusals(L):
         assert attn(L, **{name: C.c_void_p(264)}) == 1, name
     for kw in (dict(hd=80), dict(nq=7), dict(nkv=0), dict(width=0), dict(win=-1), dict(longest=-1), dict(s_max=0),
                dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("nan")), dict(qs=1023), dict(qs=1000),
-               dict(bytes=4 * 8 * 2 * 130 * 4 - 1), dict(slots=-1), dict(slots=0)):
+               dict(bytes=4 * 8 * 2 * 132 * 4 - 1), dict(slots=-1), dict(slots=0)):
         assert attn(L, **kw) == 2, kw
     assert attn(L, s_max=257) == 4 and attn(L, shift=31) == 4
 
 
 def test_attention_plan(L):
     size = L.bq_paged_attention_workspace_size
-    assert size(4, 8, 128, 1) == 0 and size(4, 8, 128, 2) == 4 * 8 * 2 * 130 * 4 and size(0, 8, 128, 2) == 0
+    assert size(4, 8, 128, 1) == 0 and size(4, 8, 128, 2) == 4 * 8 * 2 * 132 * 4 and size(0, 8, 128, 2) == 0
     for n, nq, nkv, hd, longest, win in ((1, 16, 8, 256, 1500, 1024), (64, 32, 8, 128, 16384, 0), (1, 1, 1, 64, 1, 0),
                                          (3, 8, 1, 512, 2**31 - 1, 0), (1, 16, 2, 512, 50, 7)):
         s = L.bq_paged_attention_splits(n, nq, nkv, hd, longest, win)
