@@ -7,17 +7,22 @@
 //
 // A page's reference count is the number of table entries (of any table over the
 // pool) that hold it; 0 is free.  A reorder, in terms of whole tables:
-//   1. k_reorder_tables: every sequence takes its parent's entries (in place: a
-//      workgroup owns all rows of a few columns), and the counts follow.
-//   2. k_reorder_plan (one workgroup, which does small tables too): the page a sequence writes next has to be
-//      its own.  Of the sequences on one such page, in their order, all but the
-//      last leave it for a fresh page while anyone else holds it; fresh pages are
-//      the lowest free numbers in the order (sequence, page).
-//   3. k_cache_copy: the rows already on a page that was left, in every array.
-// All counts are integers, so the order of the atomics leaves no trace.
+//   1. Every sequence takes its parent's entries, and the counts follow: an old entry
+//      counts once for each child that keeps it instead of once.
+//   2. The page a sequence writes next has to be its own.  Of the sequences on one
+//      such page, in their order, all but the last leave it for a fresh page while
+//      anyone else holds it; fresh pages are the lowest free numbers in the order
+//      (sequence, page).
+//   3. The rows already on a page that was left are copied in every array.
+// All counts are integers, so the order of atomics leaves no trace.
+//
+// Pools whose tables and counts fit LDS (k_reorder_plan<true>, k_compact<true>) take one
+// launch: every workgroup works the whole plan out for itself from the old state, marks
+// that it has read it, and copies its share; the last to mark writes the new state.
+// Larger ones are planned by launches of their own, then copied (k_cache_copy).
 #include <algorithm>
 
-#include "bq_device.hpp"
+#include "bq_half.hpp"
 #include "bq_kernels.hpp"
 #include "bq_pages.hpp"
 
@@ -25,18 +30,20 @@ namespace bq {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kWaves = kPlanThreads / 64;
 constexpr int kTableThreads = 512;
 constexpr int kBatch = 8;           // loads of a thread that are on their way at once
 constexpr int kOwned = 2048;        // wanted pages whose sequences k_reorder_plan lists
 constexpr int kTileEntries = 1024;  // table entries of a k_reorder_tables workgroup
-constexpr int64_t kOneBytes = 52000;  // tables and counts that k_reorder_plan<true> keeps in LDS
+constexpr int64_t kOneMoves = 64 << 20;  // bytes that a one-launch compaction may have to move
+constexpr int64_t kOneBytes = 128 << 10;  // tables and counts of a one-launch plan (LDS)
 
 struct CopyItem {
   int32_t src, dst, rows, pad;
 };
 
-// workspace: header {copies, 0, 0, 0}, then the copies
+// workspace: the marks of a launch's workgroups, or the plan for the next launch
+constexpr int kMaxPlanBlocks = 256;
 struct CopyList {
   int32_t count, pad[3];
   CopyItem item[1];
@@ -50,7 +57,7 @@ __device__ inline int block_scan(int v, int* wsum, int* sum) {
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     const int x = wsum[w];
     before += w < wave ? x : 0;
     all += x;
@@ -111,10 +118,11 @@ __device__ inline void load_tile(const ReorderArgs& a, int32_t* tile, int j0, in
   }
 }
 
-// ... and the new entries and counts from there: an old entry counts once for each
-// child that keeps it instead of once
-__device__ inline void store_tile(const ReorderArgs& a, int32_t* refs, const SeqLds* seq,
-                                  const int32_t* tile, int j0, int width, int threads) {
+// ... and the counts and new entries (row bases) from there, the latter to `to` with rows
+// `to_width` apart
+__device__ inline void new_tile(const ReorderArgs& a, int32_t* refs, const SeqLds* seq,
+                                const int32_t* tile, int32_t* to, int to_width, int j0, int width,
+                                int threads) {
   for (int e = threadIdx.x; e < a.num_seqs * width; e += threads) {
     const int s = e / width, c = e - s * width, j = j0 + c;
     const SeqLds q = seq[s];
@@ -123,7 +131,22 @@ __device__ inline void store_tile(const ReorderArgs& a, int32_t* refs, const Seq
       if (d) atomicAdd(&refs[tile[e]], d);
     }
     const int page = seq_keeps(plan_of(q), j) ? tile[q.parent * width + c] : -1;
-    a.base_rows[(int64_t)s * a.max_pages + j] = page >= 0 ? page << a.page_shift : -1;
+    to[(int64_t)s * to_width + j] = page >= 0 ? page << a.page_shift : -1;
+  }
+}
+
+// the pool's counts to LDS, four past the last page's as held
+__device__ inline void load_refs(const int32_t* from, int32_t* refs, int pages, int pages4) {
+  for (int q0 = threadIdx.x; q0 < pages4; q0 += kBatch * kPlanThreads) {
+    int32_t r[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int q = q0 + u * kPlanThreads;
+      r[u] = q < pages ? from[q] : 1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (q0 + u * kPlanThreads < pages4) refs[q0 + u * kPlanThreads] = r[u];
   }
 }
 
@@ -137,44 +160,85 @@ __global__ __launch_bounds__(kTableThreads) void k_reorder_tables(ReorderArgs a,
   __syncthreads();
   count_children(a, seq, kTableThreads);
   __syncthreads();
-  store_tile(a, a.refs, seq, tile, j0, width, kTableThreads);
+  new_tile(a, a.refs, seq, tile, a.base_rows, a.max_pages, j0, width, kTableThreads);
 }
 
-// ONE: the whole reorder's bookkeeping, with tables and counts in LDS; else what
-// k_reorder_tables leaves to do.
+// Rows of pages in every array: a work item is kSegment bytes of one copy of one
+// array, four 16-byte loads a thread ahead of its stores, which go past the caches (127
+// MB in copies of 0 to 256 KiB: 54 us, 4.7 TB/s; through them 60).  Items are ordered by
+// segment first, then by array: the missing ones of short copies and the small ones of
+// narrow arrays come one after the other, and no workgroup gets more of them than another
+// (66 us the other way round).  More workgroups than run at once
+// gain 1 us there, and cost a call without copies 1.5.
+constexpr int64_t kSegment = 32768;
+constexpr int kCopyBlocks = 2048;
+
+template <typename W, int THREADS>
+__device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
+  constexpr int U = 4;
+  const int n = (int)(bytes / (int64_t)sizeof(W));
+  W* dw = reinterpret_cast<W*>(d);
+  const W* sw = reinterpret_cast<const W*>(s);
+  for (int k = threadIdx.x; k < n; k += THREADS * U) {
+    W w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u * THREADS < n) w[u] = sw[k + u * THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u * THREADS < n) __builtin_nontemporal_store(w[u], dw + k + u * THREADS);
+  }
+}
+
+// share `share` of `shares` of the copies
+template <int THREADS>
+__device__ inline void copy_share(const CacheArrays& arrays, const CopyItem* items, int copies,
+                                  int segments, int share, int shares) {
+  const int64_t pairs = (int64_t)copies * arrays.n, total = pairs * segments;
+  for (int64_t w = share; w < total; w += shares) {
+    const int segment = (int)(w / pairs), r = (int)(w - segment * pairs);
+    const int array = r / copies;
+    const CopyItem it = items[r - array * copies];
+    const int64_t row = arrays.row_bytes[array];
+    uint8_t* data = static_cast<uint8_t*>(arrays.data[array]);
+    const int64_t at = segment * kSegment, bytes = (int64_t)it.rows * row;
+    if (at >= bytes) continue;
+    const int64_t len = bytes - at < kSegment ? bytes - at : kSegment;
+    uint8_t* d = data + it.dst * row + at;
+    const uint8_t* s = data + it.src * row + at;
+    const uint64_t align = reinterpret_cast<uint64_t>(data) | (uint64_t)row;
+    if ((align & 15) == 0) copy_bytes<v4i, THREADS>(d, s, len);
+    else if ((align & 3) == 0) copy_bytes<uint32_t, THREADS>(d, s, len);
+    else copy_bytes<uint8_t, THREADS>(d, s, len);
+  }
+}
+
+// ONE: the whole reorder, tables and counts in LDS and the copies too; else what
+// k_reorder_tables leaves to plan.
 template <bool ONE>
-__global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
+__global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a, CacheArrays arrays,
+                                                               int segments) {
   extern __shared__ __align__(16) int32_t lds[];
+  const int n = a.num_seqs, i = threadIdx.x, entries = n * a.max_pages;
   const int pages4 = (a.num_pages + 3) & ~3;
-  int32_t* refs = ONE ? lds : a.refs;                               // [num_pages]
-  SeqLds* seq = reinterpret_cast<SeqLds*>(lds + (ONE ? pages4 : 0));  // [num_seqs]
-  int32_t* tile = reinterpret_cast<int32_t*>(seq + a.num_seqs);     // ONE: [num_seqs][max_pages]
-  __shared__ int wsum[kPlanThreads / 64];
+  int32_t* refs = ONE ? lds : a.refs;                                 // [num_pages]
+  CopyItem* items = ONE ? reinterpret_cast<CopyItem*>(lds + pages4)   // [num_seqs]
+                        : static_cast<CopyList*>(a.workspace)->item;
+  SeqLds* seq = ONE ? reinterpret_cast<SeqLds*>(items + n) : reinterpret_cast<SeqLds*>(lds);
+  int32_t* tile = reinterpret_cast<int32_t*>(seq + n);                // ONE: [num_seqs][max_pages]
+  int32_t* rows = ONE ? tile + entries : a.base_rows;                 // the new table, as wide
+  __shared__ int wsum[kWaves], said;
   __shared__ __align__(16) int32_t last[kMaxCacheSeqs];
-  __shared__ int32_t offset[kMaxCacheSeqs + 1];
+  __shared__ int32_t offset[kMaxCacheSeqs + 1], given[kMaxCacheSeqs];
   __shared__ int16_t owner[kOwned];
-  __shared__ int ncopy;
-  CopyList* list = static_cast<CopyList*>(a.workspace);
-  const int n = a.num_seqs, i = threadIdx.x;
-  if (i == 0) ncopy = 0;
   load_seqs(a, seq, kPlanThreads);
   if constexpr (ONE) {
     load_tile(a, tile, 0, a.max_pages, kPlanThreads);
-    for (int q0 = i; q0 < pages4; q0 += kBatch * kPlanThreads) {
-      int32_t r[kBatch];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int q = q0 + u * kPlanThreads;
-        r[u] = q < a.num_pages ? a.refs[q] : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (q0 + u * kPlanThreads < pages4) refs[q0 + u * kPlanThreads] = r[u];
-    }
+    load_refs(a.refs, refs, a.num_pages, pages4);
     __syncthreads();
     count_children(a, seq, kPlanThreads);
     __syncthreads();
-    store_tile(a, refs, seq, tile, 0, a.max_pages, kPlanThreads);
+    new_tile(a, refs, seq, tile, rows, a.max_pages, 0, a.max_pages, kPlanThreads);
   }
   SeqPlan p{};
   int page = -1;
@@ -189,8 +253,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
     }
   }
   last[i] = page;
+  given[i] = -1;
   __syncthreads();  // every length has been read, every count changed
-  if (i < n) a.lens[i] = p.len;
+  if (!ONE && i < n) a.lens[i] = p.len;
   bool leaves = false;
   if (page >= 0) {
     int earlier = 0;
@@ -227,13 +292,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
         else hi = mid - 1;
       }
     }
-    const SeqPlan s = plan_of(seq[lo]);
-    const int j = s.end - (offset[lo + 1] - k);
-    a.base_rows[(int64_t)lo * a.max_pages + j] = page_ >= 0 ? page_ << a.page_shift : -1;
-    const int rows = s.len & ((1 << a.page_shift) - 1);
-    if (page_ >= 0 && j == s.full && last[lo] >= 0 && rows)
-      list->item[atomicAdd(&ncopy, 1)] =
-          CopyItem{last[lo] << a.page_shift, page_ << a.page_shift, rows, 0};
+    const int j = seq[lo].end - (offset[lo + 1] - k);
+    rows[(int64_t)lo * a.max_pages + j] = page_ >= 0 ? page_ << a.page_shift : -1;
+    if (j == seq[lo].full) given[lo] = page_;
   };
   // the first `total` free pages, lowest numbers first, four a thread
   int got = 0;
@@ -258,29 +319,53 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a) {
   if (got > total) got = total;
   for (int k = got + i; k < total; k += kPlanThreads) give(k, -1);  // no page left for these
   __syncthreads();
-  if constexpr (ONE)
-    for (int q = i; q < a.num_pages; q += kPlanThreads) a.refs[q] = refs[q];
-  if (i == 0) {
-    list->count = ncopy;
-    a.info[0] = got;
-    a.info[1] = ncopy;
-    a.info[2] = total - got;
-    a.info[3] = 0;
+  // what a left page held goes to the page that was given instead
+  const int held = p.len & ((1 << a.page_shift) - 1);
+  const int copy = leaves && held && given[i] >= 0;
+  int copies;
+  const int at = block_scan(copy, wsum, &copies) - copy;
+  if (copy) items[at] = CopyItem{page << a.page_shift, given[i] << a.page_shift, held, 0};
+  const bool done = !ONE || last_of(static_cast<uint64_t*>(a.workspace), 1, gridDim.x, blockIdx.x,
+                                    a.tag, &said);
+  if (done) {
+    if constexpr (ONE) {
+      for (int q = i; q < a.num_pages; q += kPlanThreads) a.refs[q] = refs[q];
+      for (int e = i; e < entries; e += kPlanThreads) a.base_rows[e] = rows[e];
+      if (i < n) a.lens[i] = p.len;
+    }
+    if (i == 0) {
+      if constexpr (!ONE) static_cast<CopyList*>(a.workspace)->count = copies;
+      a.info[0] = got;
+      a.info[1] = copies;
+      a.info[2] = total - got;
+      a.info[3] = 0;
+    }
   }
+  if constexpr (ONE)  // last_of's barriers stand between the items and this
+    copy_share<kPlanThreads>(arrays, items, copies, segments, blockIdx.x, gridDim.x);
 }
 
-// Page numbers after packing: with `live` pages held, the i-th free page below
-// `live` takes the i-th held page from `live` on.
-__global__ __launch_bounds__(kPlanThreads) void k_compact_plan(CompactArgs a) {
-  __shared__ int wsum[kPlanThreads / 64];
-  const int i = threadIdx.x;
-  CopyList* list = static_cast<CopyList*>(a.workspace);
-  int32_t* to = reinterpret_cast<int32_t*>(list->item + (a.num_pages / 2 + 1));
+// Packing: with `live` pages held, the i-th free page below `live` takes the i-th held
+// page from `live` on.  ONE: all of it, the plan in LDS; else the plan alone.
+template <bool ONE>
+__global__ __launch_bounds__(kPlanThreads) void k_compact(CompactArgs a, CacheArrays arrays,
+                                                          int segments) {
+  extern __shared__ __align__(16) int32_t lds[];
+  __shared__ int wsum[kWaves], said;
+  const int i = threadIdx.x, pages4 = (a.num_pages + 3) & ~3;
+  int32_t* refs = ONE ? lds : a.refs;  // [num_pages]
+  CopyItem* items = ONE ? reinterpret_cast<CopyItem*>(lds + pages4)  // [num_pages / 2 + 1]
+                        : static_cast<CopyList*>(a.workspace)->item;
+  int32_t* to = reinterpret_cast<int32_t*>(items + (a.num_pages / 2 + 1));  // [num_pages]
+  if constexpr (ONE) {
+    load_refs(a.refs, refs, a.num_pages, pages4);
+    __syncthreads();
+  }
   auto held4 = [&](int q) {  // which of four pages are held, as bits
     int m = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (q + u < a.num_pages && a.refs[q + u] != 0) m |= 1 << u;
+      if (q + u < a.num_pages && refs[q + u] != 0) m |= 1 << u;
     return m;
   };
   int mine = 0, live;
@@ -297,8 +382,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_compact_plan(CompactArgs a) {
     int kh = holes + (before & 0xFFFF), km = movers + (before >> 16);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (hole >> u & 1) list->item[kh++].dst = q + u;
-      if (mover >> u & 1) list->item[km++].src = q + u;
+      if (hole >> u & 1) items[kh++].dst = q + u;
+      if (mover >> u & 1) items[km++].src = q + u;
       if (u < in) to[q + u] = q + u;
     }
     holes += both & 0xFFFF;
@@ -306,45 +391,34 @@ __global__ __launch_bounds__(kPlanThreads) void k_compact_plan(CompactArgs a) {
   }
   __syncthreads();
   for (int k = i; k < movers; k += kPlanThreads) {
-    const int src = list->item[k].src, dst = list->item[k].dst;
+    const int src = items[k].src, dst = items[k].dst;
     to[src] = dst;
-    a.refs[dst] = a.refs[src];
-    a.refs[src] = 0;
-    list->item[k] = CopyItem{src << a.page_shift, dst << a.page_shift, 1 << a.page_shift, 0};
+    refs[dst] = refs[src];
+    refs[src] = 0;
+    items[k] = CopyItem{src << a.page_shift, dst << a.page_shift, 1 << a.page_shift, 0};
   }
-  if (i == 0) {
-    list->count = movers;
-    a.info[0] = live;
-    a.info[1] = movers;
-    a.info[2] = a.info[3] = 0;
+  // The last to have read the counts writes; were two to write, the second would find
+  // every entry where it belongs.
+  const bool done = !ONE || last_of(static_cast<uint64_t*>(a.workspace), 1, gridDim.x, blockIdx.x,
+                                    a.tag, &said);
+  if (done) {
+    if constexpr (ONE) {
+      for (int q = i; q < a.num_pages; q += kPlanThreads) a.refs[q] = refs[q];
+      if (movers)
+        for (int e = i; e < a.num_seqs * a.max_pages; e += kPlanThreads) {
+          const int page = page_number(a.base_rows[e], a.page_shift, a.num_pages);
+          if (page >= live) a.base_rows[e] = to[page] << a.page_shift;
+        }
+    }
+    if (i == 0) {
+      if constexpr (!ONE) static_cast<CopyList*>(a.workspace)->count = movers;
+      a.info[0] = live;
+      a.info[1] = movers;
+      a.info[2] = a.info[3] = 0;
+    }
   }
-}
-
-// Rows of pages in every array: a work item is kSegment bytes of one copy of one
-// array, four 16-byte loads a thread ahead of its stores, which go past the caches (127
-// MB in copies of 0 to 256 KiB: 54 us, 4.7 TB/s; through them 60).  Items are ordered by
-// segment first, then by array: the missing ones of short copies and the small ones of
-// narrow arrays come one after the other, and no workgroup gets more of them than another
-// (66 us the other way round).  More workgroups than run at once
-// gain 1 us there, and cost a call without copies 1.5.
-constexpr int64_t kSegment = 32768;
-constexpr int kCopyBlocks = 2048;
-
-template <typename W>
-__device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
-  constexpr int U = 4;
-  const int n = (int)(bytes / (int64_t)sizeof(W));
-  W* dw = reinterpret_cast<W*>(d);
-  const W* sw = reinterpret_cast<const W*>(s);
-  for (int k = threadIdx.x; k < n; k += 256 * U) {
-    W w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k + u * 256 < n) w[u] = sw[k + u * 256];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k + u * 256 < n) __builtin_nontemporal_store(w[u], dw + k + u * 256);
-  }
+  if constexpr (ONE)
+    copy_share<kPlanThreads>(arrays, items, movers, segments, blockIdx.x, gridDim.x);
 }
 
 // The first `table_blocks` workgroups (compaction) carry the tables over to the new
@@ -361,71 +435,89 @@ __global__ __launch_bounds__(256) void k_cache_copy(CacheArrays arrays, const vo
     if (page >= 0) t.base_rows[e] = to[page] << t.page_shift;
     return;
   }
-  const int copies = list->count;
-  const int64_t pairs = (int64_t)copies * arrays.n, total = pairs * segments;
-  for (int64_t w = blockIdx.x - table_blocks; w < total; w += gridDim.x - table_blocks) {
-    const int segment = (int)(w / pairs), r = (int)(w - segment * pairs);
-    const int array = r / copies;
-    const CopyItem it = list->item[r - array * copies];
-    const int64_t row = arrays.row_bytes[array];
-    uint8_t* data = static_cast<uint8_t*>(arrays.data[array]);
-    const int64_t at = segment * kSegment, bytes = (int64_t)it.rows * row;
-    if (at >= bytes) continue;
-    const int64_t len = bytes - at < kSegment ? bytes - at : kSegment;
-    uint8_t* d = data + it.dst * row + at;
-    const uint8_t* s = data + it.src * row + at;
-    const uint64_t align = reinterpret_cast<uint64_t>(data) | (uint64_t)row;
-    if ((align & 15) == 0) copy_bytes<v4i>(d, s, len);
-    else if ((align & 3) == 0) copy_bytes<uint32_t>(d, s, len);
-    else copy_bytes<uint8_t>(d, s, len);
-  }
+  copy_share<256>(arrays, list->item, list->count, segments, blockIdx.x - table_blocks,
+                  gridDim.x - table_blocks);
 }
 
-hipError_t launch_copy(const CacheArrays& arrays, void* workspace, int max_items, int page_shift,
-                       hipStream_t st, const CompactArgs* t = nullptr) {
+// segments of the widest array's page
+int64_t copy_segments(const CacheArrays& arrays, int page_shift) {
   int64_t most = 0;
   for (int i = 0; i < arrays.n; ++i) most = std::max(most, arrays.row_bytes[i] << page_shift);
-  const int64_t segments = std::max<int64_t>(1, (most + kSegment - 1) / kSegment);
+  return std::max<int64_t>(1, (most + kSegment - 1) / kSegment);
+}
+
+hipError_t launch_copy(const CacheArrays& arrays, void* workspace, int max_items, int64_t segments,
+                       hipStream_t st, const CompactArgs* t = nullptr) {
   const int64_t entries = t ? (int64_t)t->num_seqs * t->max_pages : 0;
   const int64_t table_blocks = (entries + 255) / 256;
   const int64_t copies = std::min<int64_t>((int64_t)max_items * arrays.n * segments, kCopyBlocks);
-  if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
   if (copies == 0 && table_blocks == 0) return hipSuccess;
   k_cache_copy<<<(int)(table_blocks + std::max<int64_t>(copies, 1)), 256, 0, st>>>(
       arrays, workspace, (int)segments, t ? *t : CompactArgs{}, (int)table_blocks);
   return hipGetLastError();
 }
 
+// a plan of `bytes` of LDS, by a workgroup for every four pieces that there may be to copy
+template <typename K, typename A>
+hipError_t launch_one(K kernel, A a, const CacheArrays& arrays, int64_t bytes, int max_items,
+                      int64_t segments, hipStream_t st) {
+  if (bytes > 49152) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return e;
+  }
+  const int64_t blocks = std::min<int64_t>(std::min(tune().cus, kMaxPlanBlocks),
+                                           (int64_t)max_items * arrays.n * segments / 4);
+  a.tag = launch_tag();
+  kernel<<<(int)std::max<int64_t>(blocks, 1), kPlanThreads, (size_t)bytes, st>>>(a, arrays,
+                                                                               (int)segments);
+  return hipGetLastError();
+}
+
 }  // namespace
 
-size_t reorder_workspace(int num_seqs) { return 16 + (size_t)num_seqs * sizeof(CopyItem); }
+size_t reorder_workspace(int num_seqs) {
+  return std::max(16 + (size_t)num_seqs * sizeof(CopyItem), kMaxPlanBlocks * sizeof(uint64_t));
+}
 size_t compact_workspace(int num_pages) {
-  return 16 + ((size_t)num_pages / 2 + 1) * sizeof(CopyItem) + (size_t)num_pages * 4;
+  return std::max(16 + ((size_t)num_pages / 2 + 1) * sizeof(CopyItem) + (size_t)num_pages * 4,
+                  kMaxPlanBlocks * sizeof(uint64_t));
 }
 
 hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays, hipStream_t st) {
-  const size_t seqs = sizeof(SeqLds) * a.num_seqs;
-  // What fits LDS one workgroup does alone: a launch less.
-  const int64_t one = seqs + ((int64_t)a.num_seqs * a.max_pages + ((a.num_pages + 3) & ~3)) * 4;
-  if (one <= kOneBytes) {
-    k_reorder_plan<true><<<1, kPlanThreads, (size_t)one, st>>>(a);
-  } else {
-    const int cols = std::max(1, std::min(a.max_pages, kTileEntries / a.num_seqs));
-    k_reorder_tables<<<(a.max_pages + cols - 1) / cols, kTableThreads,
-                       seqs + (size_t)cols * a.num_seqs * 4, st>>>(a, cols);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    k_reorder_plan<false><<<1, kPlanThreads, seqs, st>>>(a);
-  }
-  const hipError_t e = hipGetLastError();
-  return e != hipSuccess ? e : launch_copy(arrays, a.workspace, a.num_seqs, a.page_shift, st);
+  const int64_t segments = copy_segments(arrays, a.page_shift);
+  if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
+  const int64_t seqs = (int64_t)sizeof(SeqLds) * a.num_seqs, pages4 = (a.num_pages + 3) & ~3;
+  const int64_t one = seqs + (int64_t)sizeof(CopyItem) * a.num_seqs +
+                      4 * (pages4 + 2 * (int64_t)a.num_seqs * a.max_pages);
+  if (one <= kOneBytes)
+    return launch_one(&k_reorder_plan<true>, a, arrays, one, a.num_seqs, segments, st);
+  const int cols = std::max(1, std::min(a.max_pages, kTileEntries / a.num_seqs));
+  k_reorder_tables<<<(a.max_pages + cols - 1) / cols, kTableThreads,
+                     (size_t)seqs + (size_t)cols * a.num_seqs * 4, st>>>(a, cols);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  k_reorder_plan<false><<<1, kPlanThreads, (size_t)seqs, st>>>(a, arrays, 0);
+  e = hipGetLastError();
+  return e != hipSuccess ? e : launch_copy(arrays, a.workspace, a.num_seqs, segments, st);
 }
 
 hipError_t launch_cache_compact(const CompactArgs& a, const CacheArrays& arrays, hipStream_t st) {
-  k_compact_plan<<<1, kPlanThreads, 0, st>>>(a);
+  const int64_t segments = copy_segments(arrays, a.page_shift);
+  if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
+  const int64_t pages4 = (a.num_pages + 3) & ~3;
+  const int64_t one = 8 * pages4 + (int64_t)sizeof(CopyItem) * (a.num_pages / 2 + 1);
+  // Where much may move, the copies of a launch of their own, in small workgroups, make up
+  // for it: 64 sequences of 2000 positions, an eighth retired, 470 MB: 117 and 121 us.
+  int64_t page = 0;
+  for (int i = 0; i < arrays.n; ++i) page += arrays.row_bytes[i] << a.page_shift;
+  if (one <= kOneBytes && page * (a.num_pages / 2) <= kOneMoves)
+    return launch_one(&k_compact<true>, a, arrays, one, a.num_pages / 2, segments, st);
+  k_compact<false><<<1, kPlanThreads, 0, st>>>(a, arrays, 0);
   const hipError_t e = hipGetLastError();
-  return e != hipSuccess ? e
-                         : launch_copy(arrays, a.workspace, a.num_pages / 2, a.page_shift, st, &a);
+  return e != hipSuccess
+             ? e
+             : launch_copy(arrays, a.workspace, a.num_pages / 2, segments, st, &a);
 }
 
 }  // namespace bq

@@ -277,11 +277,13 @@ struct ReorderArgs {
   int32_t* info;                          // [4]
   void* workspace;
   int num_seqs, max_pages, page_shift, num_pages;
+  uint64_t tag;                           // the launcher's
 };
 struct CompactArgs {
   int32_t *base_rows, *refs, *info;
   void* workspace;
   int num_seqs, max_pages, page_shift, num_pages;
+  uint64_t tag;                           // the launcher's
 };
 constexpr int kMaxBeams = 64, kMaxPicks = 64;
 struct BeamArgs {

@@ -343,7 +343,8 @@ SOME = [(torch.int8, (8, 32)), (torch.float32, (8,)), (BF, (64,)), (torch.int8, 
 
 
 @pytest.mark.parametrize("n,width,shift,spare", [(1, 1, 0, 1), (4, 9, 4, 8), (7, 70, 2, 40), (33, 5, 6, 70), (256, 12, 3, 600),
-                                                 (300, 3, 0, 900), (1024, 2, 1, 1500), (2, 3000, 1, 50)])
+                                                 (300, 3, 0, 900), (1024, 2, 1, 1500), (2, 3000, 1, 50),
+                                                 (300, 80, 1, 900), (1000, 33, 0, 5000), (5, 4000, 0, 30000)])
 def test_cache_reorder(gpu, n, width, shift, spare):
     """Several steps of forks, frees and growth, each against the page-by-page reference."""
     table, lens, refs, arrays = page_case(n + width, n, width, shift, spare, SOME)
@@ -390,7 +391,8 @@ def test_cache_reorder_short_pool_and_bad_tables(gpu):
     assert short > 0
 
 
-@pytest.mark.parametrize("n,width,shift,spare", [(1, 1, 0, 1), (5, 9, 4, 30), (64, 33, 6, 100), (40, 120, 0, 3000), (3, 2, 10, 1)])
+@pytest.mark.parametrize("n,width,shift,spare", [(1, 1, 0, 1), (5, 9, 4, 30), (64, 33, 6, 100), (40, 120, 0, 3000), (3, 2, 10, 1),
+                                                 (90, 200, 0, 9000), (300, 90, 1, 500), (6, 30, 10, 20)])
 def test_cache_compact(gpu, n, width, shift, spare):
     table, lens, refs, arrays = page_case(7 * n + width, n, width, shift, spare, SOME)
     ref = Pages(table, lens, refs, shift, arrays)

@@ -101,7 +101,8 @@ def test_cache_refusals(L):
 
     assert reorder(n=0, rows=None) == 0 and compact(n=0, rows=None) == 0
     assert reorder(lens=None) == 1 and reorder(par=None) == 1
-    assert reorder(bytes=16 + 4 * 16 - 1) == 2 and compact(bytes=16 + 17 * 16 + 32 * 4 - 1) == 2
+    assert reorder(bytes=L.bq_cache_reorder_workspace_size(4) - 1) == 2
+    assert compact(bytes=L.bq_cache_compact_workspace_size(32) - 1) == 2
     for call in (reorder, compact):
         for name in ("rows", "refs", "info", "ws", "arr"):
             assert call(**{name: None}) == 1, name
