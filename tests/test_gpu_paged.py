@@ -457,6 +457,11 @@ BEAM = [  # batch, beams, vocab, n, dtype, finished, row padding
     (1, 16, 5003, 32, HF, False, 0),
     (40, 5, 2047, 5, BF, False, 0),
     (1, 2, 1 << 20, 3, HF, False, 0),
+    (10, 13, 900, 13, HF, False, 0),      # a part for each beam
+    (4, 10, 3756, 20, HF, True, 0),
+    (2, 1, 1800, 64, torch.float32, False, 0),
+    (1, 3, 130, 64, BF, True, 2),
+    (2, 5, 6000, 64, BF, False, 1),
 ]
 
 
