@@ -288,6 +288,8 @@ int bq_beam_select(const void* logits, int64_t row_stride, int dtype, const floa
   if (eos_id < -1 || eos_id >= vocab || (finished && eos_id < 0))
     return fail(BQ_ERR_SHAPE, "bq_beam_select: eos_id %d outside [-1, vocab), or -1 with finished "
                               "beams", eos_id);
+  if (out_scores == scores || (finished && out_finished == finished))
+    return fail(BQ_ERR_INVALID, "bq_beam_select: outputs may not be the inputs");
   const int size = dtype == BQ_DT_F32 ? 4 : 2;
   if (!aligned(logits, size) || !aligned(workspace, 16))
     return fail(BQ_ERR_INVALID, "bq_beam_select: logits must be aligned to their type, workspace "

@@ -49,6 +49,10 @@ __device__ inline float quad_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// Partial sums that the attention's last workgroup joins itself, instead of a launch of
+// k_paged_merge (1 x 1024 positions: 13.8 -> 11.2 us; 16 x 8000 positions of one kv head
+// with 131 KB of them: 22.8 -> 29.7).
+constexpr int64_t kJoinBytes = 48 << 10;
 constexpr int kMlStride = 4;  // floats of workspace per split beside its sums: m, l, mark
 
 // Parts of one row joined: sums scaled from each part's maximum to the common one.
@@ -391,7 +395,9 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
   if (!last_of(marks, kMlStride / 2, rg.splits, split, a.tag,
                reinterpret_cast<int*>(sm + 2 * NW * 16)))
     return;
-  // maxima and sums to LDS, over the waves' parts; then eight splits' sums at a time
+  // Maxima and sums to LDS, over the waves' parts (kJoinBytes: there are at most 192 of
+  // them, and room for 2 NW (HD + 8) at least); then eight splits' sums at a time.
+  static_assert(kJoinBytes / (4 * HD) <= NW * LD / 2 + NW * 16, "room for the splits' m and l");
   for (int e = threadIdx.x; e < G * rg.splits; e += NW * 64) {
     const int h = e / rg.splits, i = e - h * rg.splits;
     const v2f v = load2_agent(a.ws_ml + ((row0 + h) * a.s_max + i) * kMlStride);
@@ -446,8 +452,6 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a) {
   j.store(a, row, HD, col);
 }
 
-constexpr int64_t kJoinBytes = 48 << 10;
-
 template <typename T, int HD, bool SMALL>
 hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t st) {
   constexpr int NW = 4;
@@ -474,8 +478,6 @@ hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
   const int len = a.window > 0 ? std::min(a.window, max_len) : max_len;
   const int64_t tiles = ((int64_t)len + TP - 1) / TP + (a.window > 0 ? 1 : 0);
   a.chunk_tiles = (int)std::max<int64_t>(1, (tiles + a.s_max - 1) / a.s_max);
-  // Few partial sums are joined by the attention's last workgroup, which one workgroup
-  // reads in less than a launch takes.
   const bool fused = a.s_max > 1 && (int64_t)a.s_max * std::min(16, a.gqa) * HD * 4 <= kJoinBytes;
   a.tag = fused ? launch_tag() : 0;
   const hipError_t e =
@@ -483,6 +485,7 @@ hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
   if (e != hipSuccess || a.s_max == 1 || fused) return e;
   const int rpb = 256 / (HD / 4);
   const int64_t rows = (int64_t)a.num_seqs * a.num_q;
+  if ((rows + rpb - 1) / rpb > INT32_MAX) return hipErrorInvalidValue;
   k_paged_merge<T, HD><<<(int)((rows + rpb - 1) / rpb), 256, 0, st>>>(a);
   return hipGetLastError();
 }

@@ -279,10 +279,11 @@ def test_attention_far_offsets(gpu):
             assert all(same_bits(x, cache[0][int(t[i, p >> 6]) + (p & 63)]) for x, (i, p) in zip(got, ((0, 149), (1, 69))))
 
 
-def test_attention_streams_and_graph(gpu):
+@pytest.mark.parametrize("nkv,hd", [(2, 256), (2, 512), (1, 256), (8, 64)])
+def test_attention_streams_and_graph(gpu, nkv, hd):
     """Two captured graphs with a workspace each, replayed on two streams with eager work between;
     the lengths change between replays and the graph follows."""
-    nq, nkv, hd, shift = 16, 2, 256, 4
+    nq, shift = 16, 4
     cases = [attn_case([900, 333, 0], nq, nkv, hd, BF, shift, seed=s, slack=8, poison=False) for s in (1, 2)]
     dev = [[t.cuda() for t in c] for c in cases]
     outs = [torch.zeros(3, nq * hd, dtype=BF, device="cuda") for _ in cases]
@@ -412,16 +413,17 @@ def test_cache_compact(gpu, n, width, shift, spare):
     check_pages(ref, d[0], None, d[2], da, "again")
 
 
-def test_cache_graph_replays(gpu):
-    """A captured reorder and compaction, replayed on a state that goes on."""
-    n, width, shift = 8, 12, 3
-    table, lens, refs, arrays = page_case(2, n, width, shift, 40, SOME)
+@pytest.mark.parametrize("n,width,shift,spare", [(8, 12, 3, 40), (60, 90, 1, 1500), (200, 100, 0, 9000)])
+def test_cache_graph_replays(gpu, n, width, shift, spare):
+    """A captured reorder and compaction, replayed on a state that goes on: plans of one launch with
+    little and with much LDS, and of several launches."""
+    table, lens, refs, arrays = page_case(2, n, width, shift, spare, SOME)
     ref = Pages(table, lens, refs, shift, arrays)
     d = [t.cuda() for t in (table, lens, refs)]
     da = [a.cuda() for a in arrays]
     parents, grow = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(2))
     info, info2 = (torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(2))
-    ws = torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    ws = torch.full((1 << 20,), 0xFF, dtype=torch.uint8, device="cuda")
     parents.copy_(torch.arange(n, dtype=torch.int32))
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

@@ -4,13 +4,16 @@ on good and bad tables, and invariants of the page reference the GPU tests go by
 import ctypes as C
 import os
 import random
+import re
 import shutil
+import struct
 import subprocess
 
 import pytest
 import torch
 
 from paged_cases import Pages, slot_of
+from test_kernel_registers import LIB, MAGIC, READELF
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = C.c_void_p(256)  # a non-null placeholder: validation fails before any use
@@ -118,7 +121,7 @@ def test_cache_refusals(L):
 
 def test_beam_refusals(L):
     def beam(**kw):
-        a = dict(x=P, stride=1000, dt=F32, sc=P, fin=None, b=2, k=4, v=1000, n=4, eos=-1, os=P, op=P, ot=P, of=None, ws=P,
+        a = dict(x=P, stride=1000, dt=F32, sc=C.c_void_p(512), fin=None, b=2, k=4, v=1000, n=4, eos=-1, os=P, op=P, ot=P, of=None, ws=P,
                  bytes=1 << 30, st=None)
         a.update(kw)
         return L.bq_beam_select(*a.values())
@@ -128,11 +131,45 @@ def test_beam_refusals(L):
         assert beam(**{name: None}) == 1, name
     assert beam(dt=2) == 1 and beam(x=C.c_void_p(258)) == 1 and beam(ws=C.c_void_p(264)) == 1
     assert beam(dt=BF16, x=C.c_void_p(257)) == 1
+    assert beam(sc=P) == 1 and beam(fin=P, of=P, eos=3) == 1 and b"outputs" in L.bq_last_error()
     for kw in (dict(k=0), dict(v=0), dict(n=0), dict(stride=999), dict(eos=1000), dict(eos=-2), dict(fin=P), dict(bytes=16)):
         assert beam(**kw) == 2, kw
     for kw in (dict(k=65), dict(n=65), dict(v=(1 << 20) + 1, stride=1 << 21), dict(b=1 << 20)):
         assert beam(**kw) == 4, kw
     assert L.bq_beam_select_workspace_size(0, 5) == 0 and L.bq_beam_select_workspace_size(3, 0) == 0
+
+
+@pytest.fixture(scope="module")
+def spills(tmp_path_factory):
+    """{mangled kernel name: (scratch bytes, spilled vector registers)} of the built library"""
+    if not os.path.exists(LIB) or not os.path.exists(READELF):
+        pytest.skip("no built library or no tools to read it")
+    data, found = open(LIB, "rb").read(), {}
+    path = tmp_path_factory.mktemp("objs") / "obj"
+    for at in (m.start() for m in re.finditer(MAGIC, data)):
+        p = at + len(MAGIC) + 8
+        for _ in range(struct.unpack_from("<Q", data, p - 8)[0]):
+            off, size, idlen = struct.unpack_from("<QQQ", data, p)
+            target, p = data[p + 24:p + 24 + idlen], p + 24 + idlen
+            if b"gfx950" not in target or size == 0:
+                continue
+            path.write_bytes(data[at + off:at + off + size])
+            notes = subprocess.run([READELF, "--notes", str(path)], check=True, capture_output=True, text=True).stdout
+            for k in re.split(r"\n\s+- \.", notes):
+                name = re.search(r"\.name:\s+(_Z\S+)", k)
+                if name and ".vgpr_spill_count" in k:
+                    found[name[1]] = (int(re.search(r"\.private_segment_fixed_size:\s+(\d+)", k)[1]),
+                                      int(re.search(r"\.vgpr_spill_count:\s+(\d+)", k)[1]))
+    return found
+
+
+@pytest.mark.parametrize("kernel,instances", [("k_paged_attn", 16), ("k_paged_merge", 8), ("k_rope_append", 16), ("k_beam_pick", 6),
+                                              ("k_beam_parts", 3), ("k_reorder_plan", 2), ("k_compact", 2)])
+def test_no_scratch(spills, kernel, instances):
+    """The kernels that keep tiles and accumulators in registers spill none of them."""
+    mine = {n: v for n, v in spills.items() if f"{len(kernel)}{kernel}I" in n}
+    assert len(mine) == instances, sorted(mine)
+    assert not {n: v for n, v in mine.items() if v != (0, 0)}
 
 
 HARNESS = r"""
