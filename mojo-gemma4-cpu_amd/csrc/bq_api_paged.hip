@@ -302,7 +302,6 @@ int bq_beam_select(const void* logits, int64_t row_stride, int dtype, const floa
   a.out_scores = out_scores, a.out_parents = out_parents, a.out_tokens = out_tokens;
   a.out_finished = out_finished, a.workspace = workspace;
   a.batch = batch, a.beams = beams, a.vocab = vocab, a.n = n, a.eos_id = eos_id;
-  a.parts = bq::beam_parts(vocab);
   return check_hip(bq::launch_beam_select(a, size, dtype == BQ_DT_F16, S(stream)), "beam_select");
 }
 

@@ -21,10 +21,10 @@ namespace bq {
 
 namespace {
 
-constexpr int kPart = 2048;          // logits per part
+constexpr int kPart = 2048, kSmallPart = 512;  // logits per part
 constexpr int kPickThreads = 1024, kWaves = kPickThreads / 64;
 constexpr int kListed = 1024;        // candidates ranked in LDS
-constexpr int kFusedParts = 2048;    // parts of a request that one launch does all of
+constexpr int kFusedParts = 2112;    // parts of a request that one launch does all of
 
 struct BeamPart {
   double sum;  // of e^(x - max)
@@ -96,14 +96,14 @@ __device__ inline void exp64_table(double* lds) {  // by the first 32 threads
 
 // Part `part` of a row, in 16-byte words from the aligned address at or before the
 // row's start: x[i][e] is token first + (i * 64 + lane) * N + e, -inf outside the row.
-template <typename In>
+template <typename In, int PART>
 struct PartValues {
-  static constexpr int WORDS = kPart / (64 * In::N);
+  static constexpr int WORDS = PART / (64 * In::N);
   float x[WORDS][In::N];
   int first;
   __device__ void load(const typename In::raw* row, int vocab, int part) {
     const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename In::raw));
-    first = part * kPart - lead;
+    first = part * PART - lead;
     v4u w[WORDS];
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
@@ -126,8 +126,8 @@ struct PartValues {
 };
 
 // the maximum of a part and its exponentials' sum, in lane 0
-template <typename In>
-__device__ inline BeamPart sum_part(const PartValues<In>& p, const double* table) {
+template <typename In, int PART>
+__device__ inline BeamPart sum_part(const PartValues<In, PART>& p, const double* table) {
   float m = -INFINITY;  // NaN is no candidate and adds nothing
 #pragma unroll
   for (int i = 0; i < p.WORDS; ++i)
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void k_beam_parts(BeamArgs a) {
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t r = w / a.parts;
   const bool on = r < (int64_t)a.batch * a.beams && !(a.finished && a.finished[r]);
-  PartValues<In> p;
+  PartValues<In, kPart> p;
   if (on)
     p.load(static_cast<const typename In::raw*>(a.logits) + r * a.row_stride, a.vocab,
            (int)(w - r * a.parts));
@@ -257,8 +257,8 @@ __device__ inline int pick(PickLds& s, int n, Cand bound, Each&& each) {
   return r;
 }
 
-// The largest value that at least n of a wave's values reach (each lane brings VALUES of
-// them): from the first bit of their ordered form on.
+// The largest value of 16 bits that at least n of a wave's values reach (each lane brings
+// VALUES of them): from the first bit of their ordered form on.
 template <int VALUES>
 __device__ inline float nth_of_wave(const float (&v)[VALUES], int n) {
   uint32_t key[VALUES];
@@ -268,12 +268,13 @@ __device__ inline float nth_of_wave(const float (&v)[VALUES], int n) {
     key[i] = (int)w < 0 ? ~w : w | 0x80000000u;
   }
   uint32_t nth = 0;
-  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+  for (uint32_t bit = 0x80000000u; bit > 0x8000u; bit >>= 1) {
     int reach = 0;
 #pragma unroll
     for (int i = 0; i < VALUES; ++i) reach += __popcll(__ballot(key[i] >= (nth | bit)));
     if (reach >= n) nth |= bit;
   }
+  if (nth < 0x00800000u) return -INFINITY;  // of which 16 bits would be a NaN's
   return __uint_as_float(nth & 0x80000000u ? nth & 0x7FFFFFFFu : ~nth);
 }
 
@@ -305,7 +306,7 @@ __device__ inline float nth_of_tops(PickLds& s, float top, int n) {
 }
 
 // FUSED: the parts too, one a wave; the request's last workgroup picks.
-template <typename In, bool FUSED>
+template <typename In, bool FUSED, int PART>
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
   __shared__ PickLds s;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
   if constexpr (FUSED) {
     const int place = blockIdx.x - b * blocks, id = place * kWaves + wave, k = id / a.parts;
     const bool on = id < total && !(a.finished && a.finished[row0 + k]);
-    PartValues<In> p;
+    PartValues<In, PART> p;
     if (on)
       p.load(static_cast<const typename In::raw*>(a.logits) + (row0 + k) * a.row_stride, a.vocab,
              id - k * a.parts);
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
       }
       const typename In::raw* row =
           static_cast<const typename In::raw*>(a.logits) + (row0 + k) * a.row_stride;
-      PartValues<In> p;
+      PartValues<In, PART> p;
       p.load(row, a.vocab, part);
       // what may pass, by a bound in 32 bits from below; those few are read once more
       const float least = __double2float_rd(bound.score - sc + lse - 1e-9);
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
       if (a.finished && a.finished[row0 + k]) {
         if (lane == 0) best = s.score[k];
       } else {
-        PartValues<In> p;
+        PartValues<In, PART> p;
         p.load(static_cast<const typename In::raw*>(a.logits) + (row0 + k) * a.row_stride, a.vocab,
                (int)s.part[q]);
         float x = -INFINITY;
@@ -459,33 +460,46 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
   }
 }
 
+// rows that start off a 16-byte boundary have up to 7 values ahead of their first
+int parts_of(int vocab, int part) { return (vocab + 7 + part - 1) / part; }
+
+template <typename In, int PART>
+hipError_t launch_one(BeamArgs a, hipStream_t st) {
+  const int64_t total = (int64_t)a.beams * a.parts;
+  a.tag = launch_tag();
+  a.marks = reinterpret_cast<uint64_t*>(static_cast<BeamPart*>(a.workspace) + a.batch * total);
+  k_beam_pick<In, true, PART>
+      <<<(int)(a.batch * ((total + kWaves - 1) / kWaves)), kPickThreads, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+// One launch while all of its workgroups, of sixteen parts each, run at once: 4 beams
+// 262144 tokens 21 -> 14 us.  Small parts where there is room for them; more workgroups
+// than that stream better as small ones of their own.
 template <typename In>
 hipError_t launch(BeamArgs a, hipStream_t st) {
-  const int64_t total = (int64_t)a.beams * a.parts, blocks = (total + kWaves - 1) / kWaves;
-  // One launch while all of its workgroups run at once (4 beams of 262144 tokens); more
-  // stream better as small ones of their own.
-  if (total <= kFusedParts && a.batch * blocks <= tune().cus) {
-    a.tag = launch_tag();
-    a.marks = reinterpret_cast<uint64_t*>(static_cast<BeamPart*>(a.workspace) + a.batch * total);
-    if (a.batch * blocks > INT32_MAX) return hipErrorInvalidValue;
-    k_beam_pick<In, true><<<(int)(a.batch * blocks), kPickThreads, 0, st>>>(a);
-    return hipGetLastError();
-  }
-  if ((a.batch * total + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
-  k_beam_parts<In><<<(int)((a.batch * total + 3) / 4), 256, 0, st>>>(a);
+  auto fits = [&](int parts) {
+    const int64_t total = (int64_t)a.beams * parts;
+    return total <= kFusedParts && a.batch * ((total + kWaves - 1) / kWaves) <= tune().cus;
+  };
+  a.parts = parts_of(a.vocab, kSmallPart);
+  if (fits(a.parts)) return launch_one<In, kSmallPart>(a, st);
+  a.parts = parts_of(a.vocab, kPart);
+  if (fits(a.parts)) return launch_one<In, kPart>(a, st);
+  const int64_t blocks = ((int64_t)a.batch * a.beams * a.parts + 3) / 4;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  k_beam_parts<In><<<(int)blocks, 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  k_beam_pick<In, false><<<a.batch, kPickThreads, 0, st>>>(a);
+  k_beam_pick<In, false, kPart><<<a.batch, kPickThreads, 0, st>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-// rows that start off a 16-byte boundary have up to 7 values ahead of their first
-int beam_parts(int vocab) { return (vocab + 7 + kPart - 1) / kPart; }
 // the parts, and a mark for each workgroup (there are no more of them than parts)
 size_t beam_workspace(int64_t rows, int vocab) {
-  return (size_t)rows * beam_parts(vocab) * (sizeof(BeamPart) + sizeof(uint64_t));
+  return (size_t)rows * parts_of(vocab, kSmallPart) * (sizeof(BeamPart) + sizeof(uint64_t));
 }
 
 hipError_t launch_beam_select(const BeamArgs& a, int dtype_bytes, bool f16, hipStream_t st) {

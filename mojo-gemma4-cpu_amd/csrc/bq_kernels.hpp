@@ -295,8 +295,9 @@ struct BeamArgs {
   int32_t *out_parents, *out_tokens;
   uint8_t* out_finished;                  // or null
   void* workspace;
-  int batch, beams, vocab, n, eos_id, parts;
-  uint64_t tag;                           // the launcher's
+  int batch, beams, vocab, n, eos_id;
+  int parts;                              // the launcher's: parts of a row,
+  uint64_t tag;                           // this launch's mark, and where
   uint64_t* marks;
 };
 uint64_t launch_tag();  // marks of a launch whose last workgroup goes on with what all left
@@ -308,7 +309,6 @@ size_t reorder_workspace(int num_seqs);
 size_t compact_workspace(int num_pages);
 hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays, hipStream_t st);
 hipError_t launch_cache_compact(const CompactArgs& a, const CacheArrays& arrays, hipStream_t st);
-int beam_parts(int vocab);
 size_t beam_workspace(int64_t rows, int vocab);
 hipError_t launch_beam_select(const BeamArgs& a, int dtype_bytes, bool f16, hipStream_t st);
 
