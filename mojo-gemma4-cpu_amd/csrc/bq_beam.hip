@@ -473,9 +473,9 @@ hipError_t launch_one(BeamArgs a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// One launch while all of its workgroups, of sixteen parts each, run at once: 4 beams
-// 262144 tokens 21 -> 14 us.  Small parts where there is room for them; more workgroups
-// than that stream better as small ones of their own.
+// One launch while all of its workgroups, of sixteen parts each, run at once (4 beams of
+// 262144 tokens: 15 us, two launches 21), with small parts where there is room for them
+// (large ones 17); more workgroups than that stream better as small ones of their own.
 template <typename In>
 hipError_t launch(BeamArgs a, hipStream_t st) {
   auto fits = [&](int parts) {

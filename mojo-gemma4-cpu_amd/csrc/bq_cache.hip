@@ -100,21 +100,32 @@ __device__ inline void count_children(const ReorderArgs& a, SeqLds* seq, int thr
   }
 }
 
+// kBatch strided loads of a thread, asked for together; `get` says what element e is
+template <typename Get>
+__device__ inline void ask(int32_t (&v)[kBatch], int e0, int n, int threads, Get&& get) {
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) v[u] = e0 + u * threads < n ? get(e0 + u * threads) : 0;
+}
+template <typename Put>
+__device__ inline void give_to(const int32_t (&v)[kBatch], int e0, int n, int threads, Put&& put) {
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u)
+    if (e0 + u * threads < n) put(e0 + u * threads, v[u]);
+}
+
 // columns [j0, j0 + width) of the tables: old page numbers to LDS ...
+__device__ inline int32_t tile_entry(const ReorderArgs& a, int e, int j0, int width) {
+  const int s = e / width;
+  return a.base_rows[(int64_t)s * a.max_pages + j0 + (e - s * width)];
+}
 __device__ inline void load_tile(const ReorderArgs& a, int32_t* tile, int j0, int width,
                                  int threads) {
   const int n = a.num_seqs * width;
   for (int e0 = threadIdx.x; e0 < n; e0 += kBatch * threads) {
-    int32_t base[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int e = e0 + u * threads, s = e / width;
-      base[u] = e < n ? a.base_rows[(int64_t)s * a.max_pages + j0 + (e - s * width)] : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (e0 + u * threads < n)
-        tile[e0 + u * threads] = page_number(base[u], a.page_shift, a.num_pages);
+    int32_t v[kBatch];
+    ask(v, e0, n, threads, [&](int e) { return tile_entry(a, e, j0, width); });
+    give_to(v, e0, n, threads,
+            [&](int e, int32_t base) { tile[e] = page_number(base, a.page_shift, a.num_pages); });
   }
 }
 
@@ -135,18 +146,12 @@ __device__ inline void new_tile(const ReorderArgs& a, int32_t* refs, const SeqLd
   }
 }
 
-// the pool's counts to LDS, four past the last page's as held
-__device__ inline void load_refs(const int32_t* from, int32_t* refs, int pages, int pages4) {
-  for (int q0 = threadIdx.x; q0 < pages4; q0 += kBatch * kPlanThreads) {
-    int32_t r[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int q = q0 + u * kPlanThreads;
-      r[u] = q < pages ? from[q] : 1;
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (q0 + u * kPlanThreads < pages4) refs[q0 + u * kPlanThreads] = r[u];
+// the pool's counts from element e0 on to LDS, what is past the last page as held
+__device__ inline void load_refs(const int32_t* from, int32_t* refs, int pages, int pages4, int e0) {
+  for (; e0 < pages4; e0 += kBatch * kPlanThreads) {
+    int32_t v[kBatch];
+    ask(v, e0, pages, kPlanThreads, [&](int q) { return from[q]; });
+    give_to(v, e0, pages4, kPlanThreads, [&](int q, int32_t r) { refs[q] = q < pages ? r : 1; });
   }
 }
 
@@ -163,14 +168,14 @@ __global__ __launch_bounds__(kTableThreads) void k_reorder_tables(ReorderArgs a,
   new_tile(a, a.refs, seq, tile, a.base_rows, a.max_pages, j0, width, kTableThreads);
 }
 
-// Rows of pages in every array: a work item is kSegment bytes of one copy of one
-// array, four 16-byte loads a thread ahead of its stores, which go past the caches (127
+// Rows of pages in every array: a work item is a segment of one copy of one array,
+// four 16-byte loads a thread ahead of its stores, which go past the caches (127
 // MB in copies of 0 to 256 KiB: 54 us, 4.7 TB/s; through them 60).  Items are ordered by
 // segment first, then by array: the missing ones of short copies and the small ones of
 // narrow arrays come one after the other, and no workgroup gets more of them than another
 // (66 us the other way round).  More workgroups than run at once
 // gain 1 us there, and cost a call without copies 1.5.
-constexpr int64_t kSegment = 32768;
+__host__ __device__ constexpr int64_t segment_bytes(int threads) { return threads == 256 ? 32768 : 65536; }
 constexpr int kCopyBlocks = 2048;
 
 template <typename W, int THREADS>
@@ -190,7 +195,8 @@ __device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
   }
 }
 
-// share `share` of `shares` of the copies
+// share `share` of `shares` of the copies, in segments of 128 bytes a thread (64 in the
+// large workgroups' own)
 template <int THREADS>
 __device__ inline void copy_share(const CacheArrays& arrays, const CopyItem* items, int copies,
                                   int segments, int share, int shares) {
@@ -201,9 +207,9 @@ __device__ inline void copy_share(const CacheArrays& arrays, const CopyItem* ite
     const CopyItem it = items[r - array * copies];
     const int64_t row = arrays.row_bytes[array];
     uint8_t* data = static_cast<uint8_t*>(arrays.data[array]);
-    const int64_t at = segment * kSegment, bytes = (int64_t)it.rows * row;
+    const int64_t at = segment * segment_bytes(THREADS), bytes = (int64_t)it.rows * row;
     if (at >= bytes) continue;
-    const int64_t len = bytes - at < kSegment ? bytes - at : kSegment;
+    const int64_t len = bytes - at < segment_bytes(THREADS) ? bytes - at : segment_bytes(THREADS);
     uint8_t* d = data + it.dst * row + at;
     const uint8_t* s = data + it.src * row + at;
     const uint64_t align = reinterpret_cast<uint64_t>(data) | (uint64_t)row;
@@ -229,16 +235,28 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a, Ca
   int32_t* rows = ONE ? tile + entries : a.base_rows;                 // the new table, as wide
   __shared__ int wsum[kWaves], said;
   __shared__ __align__(16) int32_t last[kMaxCacheSeqs];
-  __shared__ int32_t offset[kMaxCacheSeqs + 1], given[kMaxCacheSeqs];
+  __shared__ int32_t offset[kMaxCacheSeqs + 1], given[kMaxCacheSeqs], early[kMaxCacheSeqs];
   __shared__ int16_t owner[kOwned];
-  load_seqs(a, seq, kPlanThreads);
-  if constexpr (ONE) {
-    load_tile(a, tile, 0, a.max_pages, kPlanThreads);
-    load_refs(a.refs, refs, a.num_pages, pages4);
+  early[i] = 0;
+  if constexpr (ONE) {  // all first loads before any is used
+    int32_t base[kBatch], count[kBatch];
+    ask(base, i, entries, kPlanThreads, [&](int e) { return tile_entry(a, e, 0, a.max_pages); });
+    ask(count, i, a.num_pages, kPlanThreads, [&](int q) { return a.refs[q]; });
+    load_seqs(a, seq, kPlanThreads);
+    give_to(base, i, entries, kPlanThreads, [&](int e, int32_t v) {
+      tile[e] = page_number(v, a.page_shift, a.num_pages);
+    });
+    give_to(count, i, pages4, kPlanThreads,
+            [&](int q, int32_t r) { refs[q] = q < a.num_pages ? r : 1; });
+    for (int e = i + kBatch * kPlanThreads; e < entries; e += kPlanThreads)
+      tile[e] = page_number(tile_entry(a, e, 0, a.max_pages), a.page_shift, a.num_pages);
+    load_refs(a.refs, refs, a.num_pages, pages4, i + kBatch * kPlanThreads);
     __syncthreads();
     count_children(a, seq, kPlanThreads);
     __syncthreads();
     new_tile(a, refs, seq, tile, rows, a.max_pages, 0, a.max_pages, kPlanThreads);
+  } else {
+    load_seqs(a, seq, kPlanThreads);
   }
   SeqPlan p{};
   int page = -1;
@@ -256,18 +274,24 @@ __global__ __launch_bounds__(kPlanThreads) void k_reorder_plan(ReorderArgs a, Ca
   given[i] = -1;
   __syncthreads();  // every length has been read, every count changed
   if (!ONE && i < n) a.lens[i] = p.len;
-  bool leaves = false;
-  if (page >= 0) {
+  // earlier sequences on the same page, counted by 1024 / n threads each
+  int np = 64;
+  while (np < n) np <<= 1;
+  {
+    const int who = i & (np - 1), step = 4 * (kPlanThreads / np), mine = last[who];
     int earlier = 0;
-#pragma unroll 4
-    for (int k = 0; k < (i & ~3); k += 4) {
-      const v4i l = *reinterpret_cast<const v4i*>(last + k);
+    if (mine >= 0)
+#pragma unroll 2
+      for (int k = 4 * (i / np); k < who; k += step) {
+        const v4i l = *reinterpret_cast<const v4i*>(last + k);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) earlier += l[u] == page;
-    }
-    for (int k = i & ~3; k < i; ++k) earlier += last[k] == page;
-    leaves = refs[page] - earlier > 1;
+        for (int u = 0; u < 4; ++u) earlier += l[u] == mine && k + u < who;
+      }
+    if (earlier) atomicAdd(&early[who], earlier);
   }
+  __syncthreads();
+  const bool leaves = page >= 0 && refs[page] - early[i] > 1;
+  __syncthreads();  // before counts fall
   int fresh = i < n ? p.end - p.full : 0;
   if (page >= 0 && !leaves) --fresh;
   int total;
@@ -358,7 +382,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_compact(CompactArgs a, CacheAr
                         : static_cast<CopyList*>(a.workspace)->item;
   int32_t* to = reinterpret_cast<int32_t*>(items + (a.num_pages / 2 + 1));  // [num_pages]
   if constexpr (ONE) {
-    load_refs(a.refs, refs, a.num_pages, pages4);
+    load_refs(a.refs, refs, a.num_pages, pages4, i);
     __syncthreads();
   }
   auto held4 = [&](int q) {  // which of four pages are held, as bits
@@ -440,10 +464,11 @@ __global__ __launch_bounds__(256) void k_cache_copy(CacheArrays arrays, const vo
 }
 
 // segments of the widest array's page
-int64_t copy_segments(const CacheArrays& arrays, int page_shift) {
+int64_t copy_segments(const CacheArrays& arrays, int page_shift, int threads) {
   int64_t most = 0;
   for (int i = 0; i < arrays.n; ++i) most = std::max(most, arrays.row_bytes[i] << page_shift);
-  return std::max<int64_t>(1, (most + kSegment - 1) / kSegment);
+  const int64_t each = segment_bytes(threads);
+  return std::max<int64_t>(1, (most + each - 1) / each);
 }
 
 hipError_t launch_copy(const CacheArrays& arrays, void* workspace, int max_items, int64_t segments,
@@ -457,17 +482,17 @@ hipError_t launch_copy(const CacheArrays& arrays, void* workspace, int max_items
   return hipGetLastError();
 }
 
-// a plan of `bytes` of LDS, by a workgroup for every four pieces that there may be to copy
+// a plan of `bytes` of LDS, by a workgroup for every two pieces that there may be to copy
 template <typename K, typename A>
 hipError_t launch_one(K kernel, A a, const CacheArrays& arrays, int64_t bytes, int max_items,
                       int64_t segments, hipStream_t st) {
-  if (bytes > 49152) {
+  if (bytes > 40960) {  // with 20 KiB of fixed LDS
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != hipSuccess) return e;
   }
   const int64_t blocks = std::min<int64_t>(std::min(tune().cus, kMaxPlanBlocks),
-                                           (int64_t)max_items * arrays.n * segments / 4);
+                                           (int64_t)max_items * arrays.n * segments / 2);
   a.tag = launch_tag();
   kernel<<<(int)std::max<int64_t>(blocks, 1), kPlanThreads, (size_t)bytes, st>>>(a, arrays,
                                                                                (int)segments);
@@ -485,13 +510,14 @@ size_t compact_workspace(int num_pages) {
 }
 
 hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays, hipStream_t st) {
-  const int64_t segments = copy_segments(arrays, a.page_shift);
+  const int64_t segments = copy_segments(arrays, a.page_shift, 256);
+  const int64_t large = copy_segments(arrays, a.page_shift, kPlanThreads);
   if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
   const int64_t seqs = (int64_t)sizeof(SeqLds) * a.num_seqs, pages4 = (a.num_pages + 3) & ~3;
   const int64_t one = seqs + (int64_t)sizeof(CopyItem) * a.num_seqs +
                       4 * (pages4 + 2 * (int64_t)a.num_seqs * a.max_pages);
   if (one <= kOneBytes)
-    return launch_one(&k_reorder_plan<true>, a, arrays, one, a.num_seqs, segments, st);
+    return launch_one(&k_reorder_plan<true>, a, arrays, one, a.num_seqs, large, st);
   const int cols = std::max(1, std::min(a.max_pages, kTileEntries / a.num_seqs));
   k_reorder_tables<<<(a.max_pages + cols - 1) / cols, kTableThreads,
                      (size_t)seqs + (size_t)cols * a.num_seqs * 4, st>>>(a, cols);
@@ -503,7 +529,8 @@ hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays,
 }
 
 hipError_t launch_cache_compact(const CompactArgs& a, const CacheArrays& arrays, hipStream_t st) {
-  const int64_t segments = copy_segments(arrays, a.page_shift);
+  const int64_t segments = copy_segments(arrays, a.page_shift, 256);
+  const int64_t large = copy_segments(arrays, a.page_shift, kPlanThreads);
   if (segments * kMaxCacheArrays > INT32_MAX) return hipErrorInvalidValue;
   const int64_t pages4 = (a.num_pages + 3) & ~3;
   const int64_t one = 8 * pages4 + (int64_t)sizeof(CopyItem) * (a.num_pages / 2 + 1);
@@ -512,7 +539,7 @@ hipError_t launch_cache_compact(const CompactArgs& a, const CacheArrays& arrays,
   int64_t page = 0;
   for (int i = 0; i < arrays.n; ++i) page += arrays.row_bytes[i] << a.page_shift;
   if (one <= kOneBytes && page * (a.num_pages / 2) <= kOneMoves)
-    return launch_one(&k_compact<true>, a, arrays, one, a.num_pages / 2, segments, st);
+    return launch_one(&k_compact<true>, a, arrays, one, a.num_pages / 2, large, st);
   k_compact<false><<<1, kPlanThreads, 0, st>>>(a, arrays, 0);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess
