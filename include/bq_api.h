@@ -577,7 +577,8 @@ size_t bq_paged_attention_workspace_size(int num_seqs, int num_q, int head_dim, 
  * take no part is not looked at.  out [num_seqs, num_q * head_dim] (zeros where
  * nothing takes part), lse [num_seqs, num_q] (may be NULL) the natural logarithm
  * of the sum of exponentials (-inf there).  Scores, softmax and sums are 32
- * bits; the weights are rounded to the cache's type for the product with v.
+ * bits; the weights meet v as two values of the cache's type, the second what the
+ * first leaves.
  * kv_lens may hold more than max_kv_len, which only sizes the splits.
  * num_q % num_kv == 0; head_dim in {64, 128, 256, 512}; s_max in [1, 256]; q,
  * caches, out and workspace 16-byte aligned, q_stride a multiple of 8;

@@ -19,9 +19,10 @@
 // transposed, as O^T = V^T P^T: a lane reads 8 columns of its positions (16 lanes:
 // 256 contiguous bytes of a row) and pairs positions with one byte permute per
 // two values.  No LDS and no cross-lane traffic but the maxima.
-// Weights are rounded to the cache's type for that product (each by 2^-9 or 2^-12
-// of itself; their sum is taken from the unrounded ones in 32 bits); scores,
-// maxima, sums and outputs are 32 bits until the one rounding at the end.
+// Weights go to that product as two values of the cache's type, the second what
+// rounding the first leaves (2^-16 or 2^-22 of the weight are lost; one value alone
+// would cost as much again as the output's own rounding, and saves 1% of the time);
+// scores, maxima, sums and outputs are 32 bits until the one rounding at the end.
 //
 // The waves of a workgroup take every NW-th tile of a range and join in LDS; the ranges
 // of a sequence are joined in their order, by the last of its workgroups or, where that
@@ -184,11 +185,11 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
 #pragma unroll
   for (int r = 0; r < 4; ++r) voff[r] = (uint32_t)((quad * 4 + r) * stride + n16 * CPL) * 2;
 
-  // a tile's rows: its slots (SMALL: of this lane's rows; else of the first row of each
+  // a tile's rows: its slots (SMALL: of position lane % TP; else of the first row of each
   // 16, the same in all lanes) and which of its positions take part
   struct Tile {
     uint32_t ok;
-    int32_t slot[SMALL ? MT + NP : MT];
+    int32_t slot[SMALL ? 1 : MT];
   };
   auto find = [&](int t) {
     Tile x;
@@ -198,12 +199,7 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
       const bool in = p >= rg.start && p < rg.len;
       const int64_t s = in ? page_slot(rows, a.max_pages, a.page_shift, a.num_slots, p) : -1;
       x.ok = (uint32_t)__ballot(s >= 0) & FULL;
-      const int sl = s < 0 ? 0 : (int)s;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) x.slot[i] = __shfl(sl, i * 16 + n16);
-#pragma unroll
-      for (int j = 0; j < NP; ++j)
-        x.slot[MT + j] = __shfl(sl, (j >> 2) * 16 + quad * 4 + (j & 3));
+      x.slot[0] = s < 0 ? 0 : (int)s;
     } else {
       x.ok = FULL;
 #pragma unroll
@@ -227,7 +223,8 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     for (int i = 0; i < MT; ++i) {
       const char* p;
       if constexpr (SMALL)
-        p = reinterpret_cast<const char*>(kc + x.slot[i] * stride + quad * 8);
+        p = reinterpret_cast<const char*>(kc + __shfl(x.slot[0], i * 16 + n16) * stride +
+                                          quad * 8);
       else
         p = reinterpret_cast<const char*>(kc + x.slot[i] * stride) + koff;
 #pragma unroll
@@ -239,7 +236,8 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     for (int j = 0; j < NP; ++j) {
       const char* p;
       if constexpr (SMALL)
-        p = reinterpret_cast<const char*>(vc + x.slot[MT + j] * stride + n16 * CPL);
+        p = reinterpret_cast<const char*>(
+            vc + __shfl(x.slot[0], (j >> 2) * 16 + quad * 4 + (j & 3)) * stride + n16 * CPL);
       else
         p = reinterpret_cast<const char*>(vc + x.slot[j >> 2] * stride) + voff[j & 3];
 #pragma unroll
@@ -311,13 +309,14 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     const float ms = mn == -INFINITY ? 0.0f : mn;
     const float alpha = exp2_(m - ms), mw = ms - T::kWeightBits;
     m = mn;
-    uint32_t pf[NP / 2];
+    uint32_t pf[NP / 2], pl[NP / 2];  // the weights, and what rounding them leaves
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < NP; j += 2) {
       const float p0_ = exp2_(x[j] - mw), p1_ = exp2_(x[j + 1] - mw);
       sum += p0_ + p1_;
       pf[j / 2] = T::pack(p0_, p1_);
+      pl[j / 2] = T::pack(p0_ - T::lo(pf[j / 2]), p1_ - T::hi(pf[j / 2]));
     }
     l = fmaf(l, alpha, sum);
     if (cur.ok != FULL) {  // what stands in other rows may be anything
@@ -339,10 +338,15 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
         for (int j = 0; j < NP / 2; ++j)
           vt[j] = __builtin_amdgcn_perm(vf[i][2 * j + 1][c / 2], vf[i][2 * j][c / 2], sel);
         v4f32 acc = o[i][c] * alpha;
-        if constexpr (NP == 8)
-          acc = T::mfma32(v4u{vt[0], vt[1], vt[2], vt[3]}, v4u{pf[0], pf[1], pf[2], pf[3]}, acc);
-        else
-          acc = T::mfma16(v2u{vt[0], vt[1]}, v2u{pf[0], pf[1]}, acc);
+        if constexpr (NP == 8) {
+          const v4u v = {vt[0], vt[1], vt[2], vt[3]};
+          acc = T::mfma32(v, v4u{pf[0], pf[1], pf[2], pf[3]}, acc);
+          acc = T::mfma32(v, v4u{pl[0], pl[1], pl[2], pl[3]}, acc);
+        } else {
+          const v2u v = {vt[0], vt[1]};
+          acc = T::mfma16(v, v2u{pf[0], pf[1]}, acc);
+          acc = T::mfma16(v, v2u{pl[0], pl[1]}, acc);
+        }
         o[i][c] = acc;
       }
     if (more) load_v(next);
