@@ -559,13 +559,13 @@ int bq_rope_append(const void* q, const void* k, const void* v, int64_t q_stride
                    void* k_cache, void* v_cache, int num_q, int num_kv, int head_dim, int dtype,
                    int num_tokens, void* stream);
 
-/* The split count bq_paged_attention is sized for (longest sequence
- * max_kv_len; window 0: none). */
+/* The slots per sequence (s_max) that bq_paged_attention makes good use of where
+ * no sequence has more than max_kv_len positions (window 0: none). */
 int bq_paged_attention_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len,
                               int window);
 
-/* Bytes of device workspace bq_paged_attention needs for s_max splits (0 for
- * one split). */
+/* Bytes of device workspace bq_paged_attention needs for s_max slots per
+ * sequence (0 for one). */
 size_t bq_paged_attention_workspace_size(int num_seqs, int num_q, int head_dim, int s_max);
 
 /* Attention of one new token per sequence over the pages: sequence s has
@@ -579,17 +579,17 @@ size_t bq_paged_attention_workspace_size(int num_seqs, int num_q, int head_dim, 
  * of the sum of exponentials (-inf there).  Scores, softmax and sums are 32
  * bits; the weights meet v as two values of the cache's type, the second what the
  * first leaves.
- * kv_lens may hold more than max_kv_len, which only sizes the splits.
+ * The call works in num_seqs * s_max slots per kv head, which the sequences share
+ * by their lengths on the device: a long one beside short ones is split over many.
  * num_q % num_kv == 0; head_dim in {64, 128, 256, 512}; s_max in [1, 256]; q,
  * caches, out and workspace 16-byte aligned, q_stride a multiple of 8;
- * workspace >= bq_paged_attention_workspace_size(), NULL for one split.  Calls
+ * workspace >= bq_paged_attention_workspace_size(), NULL for s_max 1.  Calls
  * that overlap need a workspace each. */
 int bq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                        int64_t num_slots, const int32_t* base_rows, int max_pages, int page_shift,
                        const int32_t* kv_lens, void* out, float* lse, int num_seqs, int num_q,
                        int num_kv, int head_dim, int window, float scale, float softcap, int dtype,
-                       int max_kv_len, int s_max, void* workspace, size_t workspace_bytes,
-                       void* stream);
+                       int s_max, void* workspace, size_t workspace_bytes, void* stream);
 
 /* One array of a paged cache (host struct): num_pages << page_shift rows. */
 typedef struct bq_cache_array {

@@ -82,7 +82,7 @@ SIGNATURES = {
     "bq_paged_attention_splits": [_i] * 6,
     "bq_paged_attention_workspace_size": [_i] * 4,
     "bq_paged_attention": [_vp, _l, _vp, _vp, _l, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i,
-                           _f, _f, _i, _i, _i, _vp, _sz, _vp],
+                           _f, _f, _i, _i, _vp, _sz, _vp],
     "bq_cache_reorder_workspace_size": [_i],
     "bq_cache_reorder": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp],
     "bq_cache_compact_workspace_size": [_i],
@@ -943,7 +943,7 @@ def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv:
                     workspace=None, out=None, lse=None):
     """bq_paged_attention: one new token per sequence over the pages -> [S,
     num_q*hd] of q's type (bf16 or f16).  kv_lens int32 [S], the new token's
-    position among them.  max_kv_len sizes the splits (None: the table's);
+    position among them.  max_kv_len sizes the default s_max (None: the table's);
     scale None: head_dim ** -0.5; lse: f32 [S, num_q] to fill."""
     dt = _half(q, k_cache, v_cache, out)
     st = _here(q, k_cache, v_cache, base_rows, kv_lens, workspace, out, lse)
@@ -969,7 +969,7 @@ def paged_attention(q, k_cache, v_cache, base_rows, kv_lens, num_q: int, num_kv:
         q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), slots,
         base_rows.data_ptr(), width, page_shift, kv_lens.data_ptr(), out.data_ptr(), _ptr(lse), S,
         num_q, num_kv, head_dim, window, head_dim ** -0.5 if scale is None else scale, softcap, dt,
-        max_kv_len, s_max, _ptr(workspace),
+        s_max, _ptr(workspace),
         0 if workspace is None else workspace.nbytes, st))
     return out
 

@@ -174,8 +174,7 @@ int bq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, con
                        int64_t num_slots, const int32_t* base_rows, int max_pages, int page_shift,
                        const int32_t* kv_lens, void* out, float* lse, int num_seqs, int num_q,
                        int num_kv, int head_dim, int window, float scale, float softcap, int dtype,
-                       int max_kv_len, int s_max, void* workspace, size_t workspace_bytes,
-                       void* stream) {
+                       int s_max, void* workspace, size_t workspace_bytes, void* stream) {
   if (num_seqs <= 0) return BQ_OK;
   if (!q || !k_cache || !v_cache || !base_rows || !kv_lens || !out || (s_max > 1 && !workspace))
     return fail(BQ_ERR_INVALID, "bq_paged_attention: null pointer");
@@ -186,8 +185,8 @@ int bq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, con
   if (!hd_ok(head_dim) || num_q <= 0 || num_kv <= 0 || num_q % num_kv || num_slots <= 0)
     return fail(BQ_ERR_SHAPE, "bq_paged_attention: need head_dim in {64,128,256,512}, num_q %% "
                               "num_kv == 0, num_slots > 0");
-  if (window < 0 || max_kv_len < 0 || s_max < 1)
-    return fail(BQ_ERR_SHAPE, "bq_paged_attention: need window, max_kv_len >= 0, s_max >= 1");
+  if (window < 0 || s_max < 1)
+    return fail(BQ_ERR_SHAPE, "bq_paged_attention: need window >= 0, s_max >= 1");
   if (s_max > 256 || num_q > (1 << 16))
     return fail(BQ_ERR_UNSUPPORTED, "bq_paged_attention: s_max %d > 256 or more than 2^16 heads", s_max);
   if (!(softcap >= 0.0f) || !(scale == scale))
@@ -219,7 +218,7 @@ int bq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, con
   a.scale2 = softcap > 0.0f ? scale : scale * kLog2e;
   a.softcap2 = softcap * kLog2e;
   a.inv_cap = softcap > 0.0f ? 2.0f * kLog2e / softcap : 0.0f;
-  return check_hip(bq::launch_paged_attn(a, head_dim, max_kv_len, dtype == BQ_DT_F16, S(stream)),
+  return check_hip(bq::launch_paged_attn(a, head_dim, dtype == BQ_DT_F16, S(stream)),
                    "paged_attention");
 }
 

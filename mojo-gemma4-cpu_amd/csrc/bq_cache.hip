@@ -195,8 +195,8 @@ __device__ inline void copy_bytes(uint8_t* d, const uint8_t* s, int64_t bytes) {
   }
 }
 
-// share `share` of `shares` of the copies, in segments of 128 bytes a thread (64 in the
-// large workgroups' own)
+// share `share` of `shares` of the copies, in segments of 128 bytes a thread (64 where a
+// workgroup has 1024 threads)
 template <int THREADS>
 __device__ inline void copy_share(const CacheArrays& arrays, const CopyItem* items, int copies,
                                   int segments, int share, int shares) {

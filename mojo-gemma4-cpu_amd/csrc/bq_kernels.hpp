@@ -259,9 +259,9 @@ struct PagedAttnArgs {
   const int32_t *base_rows, *kv_lens;     // [num_seqs, max_pages], [num_seqs]
   uint16_t* out;                          // [num_seqs, num_q * head_dim]
   float* lse;                             // [num_seqs, num_q] or null
-  float *ws_acc, *ws_ml;                  // [num_seqs, num_q, s_max] x head_dim and x 4
+  float *ws_acc, *ws_ml;                  // [num_q, num_seqs * s_max] x head_dim and x 4
   int num_seqs, num_q, num_kv, gqa, head_groups, max_pages, page_shift, window, s_max;
-  int chunk_tiles;                        // the launcher's: tiles per split,
+  int units, n_max;                       // the launcher's: workgroups shared out, most splits
   uint64_t tag;                           // and this launch's mark (0: k_paged_merge joins)
   float scale2, softcap2, inv_cap;        // score factors (see bq_paged_attn.hip)
 };
@@ -303,8 +303,7 @@ struct BeamArgs {
 uint64_t launch_tag();  // marks of a launch whose last workgroup goes on with what all left
 hipError_t launch_rope_append(const RopeArgs& a, int head_dim, bool f16, hipStream_t st);
 int paged_attn_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len, int window);
-hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, int max_len, bool f16,
-                             hipStream_t st);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, bool f16, hipStream_t st);
 size_t reorder_workspace(int num_seqs);
 size_t compact_workspace(int num_pages);
 hipError_t launch_cache_reorder(const ReorderArgs& a, const CacheArrays& arrays, hipStream_t st);

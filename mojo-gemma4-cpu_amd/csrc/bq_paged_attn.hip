@@ -28,8 +28,8 @@
 // of a sequence are joined in their order, by the last of its workgroups or, where that
 // is much, by k_paged_merge.
 //
-// 64 sequences of 14 to 16 thousand positions, 8 kv heads of 128: 692 us, 5.8 TB/s (a
-// large read reaches 6.0); 16 of 4096, 2 kv heads of 512: 47 + 5 us, 4.8 TB/s.
+// 64 sequences of 14 to 16 thousand positions, 8 kv heads of 128: 697 us, 5.7 TB/s (a
+// large read reaches 6.0); 16 of 4096, 2 kv heads of 512: 49 + 5 us, 4.7 TB/s.
 #include <algorithm>
 
 #include "bq_half.hpp"
@@ -57,8 +57,13 @@ __device__ inline float quad_sum(float x) {
 // Partial sums that the attention's last workgroup joins itself, instead of a launch of
 // k_paged_merge (1 x 1024 positions: 13.8 -> 11.2 us; 16 x 8000 positions of one kv head
 // with 131 KB of them: 22.8 -> 29.7).
-constexpr int64_t kJoinBytes = 48 << 10;
+constexpr int64_t kJoinBytes = 48 << 10;  // of a sequence of mean length; twice that at most
+constexpr int kJoinMost = 128;            // splits
 constexpr int kMlStride = 4;  // floats of workspace per split beside its sums: m, l, mark
+// where there are no marks: a sequence's first slot and its splits, for k_paged_merge
+__device__ inline int2* plan_of(const PagedAttnArgs& a, int seq) {
+  return reinterpret_cast<int2*>(a.ws_ml + (int64_t)seq * kMlStride + 2);
+}
 
 // Parts of one row joined: sums scaled from each part's maximum to the common one.
 template <typename T>
@@ -84,28 +89,102 @@ struct Joined {
   }
 };
 
-// a sequence's positions and the tiles of them that split `split` takes
-struct Range {
-  int len, start;  // positions [start, len)
-  int t0, t1;      // tiles of TP positions, absolute
-  int splits;      // of this sequence
+// a sequence's positions [start, len) and its tiles [first, end) of TP positions
+struct Span {
+  int len, start, first, end;
 };
 
-__device__ inline Range attn_range(const PagedAttnArgs& a, int seq, int split, int tp) {
-  Range r;
+__device__ inline Span attn_span(const PagedAttnArgs& a, int kv_len, int tp) {
+  Span r;
   const int64_t room = (int64_t)a.max_pages << a.page_shift;
-  int64_t len = a.kv_lens[seq];
-  len = len < room ? len : room;
+  const int64_t len = kv_len < room ? kv_len : room;
   r.len = (int)(len > 0 ? len : 0);
   r.start = a.window > 0 && r.len > a.window ? r.len - a.window : 0;
-  const int first = r.start / tp, end = (r.len + tp - 1) / tp;
-  int n = (end - first + a.chunk_tiles - 1) / a.chunk_tiles;
-  r.splits = n < a.s_max ? n : a.s_max;
-  r.t0 = first + split * a.chunk_tiles;
-  // the last split takes what a sequence longer than the plan's has left
-  r.t1 = split == r.splits - 1 ? end : r.t0 + a.chunk_tiles;
-  if (split >= r.splits) r.t1 = r.t0;
+  r.first = r.start / tp, r.end = (int)(((int64_t)r.len + tp - 1) / tp);
   return r;
+}
+
+// What a workgroup takes: split `split` of the `splits` of sequence `seq` (-1: nothing),
+// whose partial sums begin at `slot0`.
+struct Work {
+  int seq, split, splits, slot0;
+  int kv_len;  // the sequence's entry
+};
+
+// Shares the slots out by length (attn_splits): 64 sequences, one of 65536 positions and
+// 63 of 512, 8 kv heads of 128: 815 us with one workgroup each, 89 shared out.  Every wave
+// works it out from the lengths, a lane for every 64th part of the sequences.  From two
+// units a sequence on, the longest split counts: the largest share that rounded up fills
+// no more than `units` (64 of 1 to 8192 positions, 4 kv heads of 256, 2 units each: 276
+// rounded down, 223).  Taking the longest first would help where long ones meet on a
+// compute unit, but every wave's sort costs as much (64 of 300: 17.6 -> 24.5 us).
+__device__ inline Work attn_work(const PagedAttnArgs& a, int slot, int tp) {
+  if (a.s_max == 1) return {slot, 0, 1, 0, a.kv_lens[slot]};
+  auto tiles = [&](int kv_len) {
+    const Span r = attn_span(a, kv_len, tp);
+    return r.end - r.first;
+  };
+  if (a.num_seqs == 1) {
+    const int t = tiles(a.kv_lens[0]);
+    const int n = attn_splits(t, t > 0 ? (double)a.units / t : 0.0, kRoundDown, a.n_max);
+    return {slot < n ? 0 : -1, slot, n, 0, a.kv_lens[0]};
+  }
+  const int lane = lane_id(), per = (a.num_seqs + 63) / 64;
+  const int s0 = min(lane * per, a.num_seqs), s1 = min(s0 + per, a.num_seqs);
+  Work w{s0, 0, 1, 0, 0};
+  auto sum = [](auto x) { return wave_all(x, [](auto p, auto q) { return p + q; }); };
+  const bool up = attn_rounds_up(a.num_seqs, a.units);
+  const double round = up ? kRoundUp : kRoundDown;
+  double share;
+  int mine = 0;
+  if (per == 1) {
+    const bool on = s0 < s1;
+    w.kv_len = on ? a.kv_lens[s0] : 0;
+    const int t = tiles(w.kv_len);
+    auto count = [&](double x) { return on ? attn_splits(t, x, round, a.n_max) : 0; };
+    const double all = sum((double)t);
+    share = all > 0.0 ? a.units / all : 0.0;
+    if (up && all > 0.0 && sum(count(share)) > a.units) {
+      double lo = (a.units - a.num_seqs) / all, hi = share;
+      for (int i = 0; i < 5; ++i) {
+        const double mid = 0.5 * (lo + hi);
+        (sum(count(mid)) <= a.units ? lo : hi) = mid;
+      }
+      share = lo;
+    }
+    w.splits = mine = count(share);
+  } else {
+    double all = 0.0;
+    for (int s = s0; s < s1; ++s) all += tiles(a.kv_lens[s]);
+    all = sum(all);
+    share = all > 0.0 ? a.units / all : 0.0;
+    for (int s = s0; s < s1; ++s) mine += attn_splits(tiles(a.kv_lens[s]), share, round, a.n_max);
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int x = __shfl_up(upto, d);
+    if (lane >= d) upto += x;
+  }
+  const uint64_t past = __ballot(upto > slot);
+  if (past == 0) return {-1, 0, 1, 0, 0};
+  const int from = __builtin_ctzll(past);
+  w.slot0 = upto - mine;
+  if (per > 1 && lane == from) {
+    for (; w.seq < s1; ++w.seq) {
+      w.kv_len = a.kv_lens[w.seq];
+      w.splits = attn_splits(tiles(w.kv_len), share, round, a.n_max);
+      if (w.slot0 + w.splits > slot) break;
+      w.slot0 += w.splits;
+    }
+    if (w.seq == s1) w.seq = -1;  // lengths that changed meanwhile
+  }
+  w.seq = __builtin_amdgcn_readlane(w.seq, from);
+  w.splits = __builtin_amdgcn_readlane(w.splits, from);
+  w.slot0 = __builtin_amdgcn_readlane(w.slot0, from);
+  w.kv_len = __builtin_amdgcn_readlane(w.kv_len, from);
+  w.split = slot - w.slot0;
+  return w;
 }
 
 // From HD = 256 on, 16 positions a tile: K, V, the queries and the accumulators of 32
@@ -155,14 +234,17 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     b = b / (8 * a.head_groups) * 8 + b % 8;
     if (b >= a.num_seqs * a.num_kv * a.s_max) return;
   }
-  const int split = b % a.s_max;
-  b /= a.s_max;
-  const int kvh = b % a.num_kv, seq = b / a.num_kv;
+  const int kvh = b % a.num_kv;
+  const Work wk = attn_work(a, b / a.num_kv, TP);
+  if (wk.seq < 0) return;
+  const int seq = wk.seq;
   const int G = min(16, a.gqa - hg * 16);
   const int head0 = kvh * a.gqa + hg * 16;
 
-  const Range rg = attn_range(a, seq, split, TP);
-  if (split > 0 && split >= rg.splits) return;  // split 0 also writes empty rows
+  const Span rg = attn_span(a, wk.kv_len, TP);
+  const int each = (rg.end - rg.first) / wk.splits, odd = (rg.end - rg.first) % wk.splits;
+  const int t0 = rg.first + wk.split * each + min(wk.split, odd);
+  const int t1 = t0 + each + (wk.split < odd ? 1 : 0);
 
   // the queries: in registers, or (large heads) in LDS for all waves
   v4u qf[KS];
@@ -262,13 +344,13 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     for (int c = 0; c < CPL; ++c) o[i][c] = v4f32{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
 
-  int t = rg.t0 + wave;
+  int t = t0 + wave;
   Tile cur{}, next{};
-  if (t < rg.t1) {
+  if (t < t1) {
     cur = find(t);
     load_k(cur);
     load_v(cur);
-    if (t + NW < rg.t1) next = find(t + NW);
+    if (t + NW < t1) next = find(t + NW);
   }
   if constexpr (QLDS) {
 #pragma unroll
@@ -276,8 +358,8 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
       if (ks % NW == wave) qs[ks * 64 + lane] = qf[ks];
     __syncthreads();
   }
-  for (; t < rg.t1; t += NW) {
-    const bool more = t + NW < rg.t1;
+  for (; t < t1; t += NW) {
+    const bool more = t + NW < t1;
     // scores in powers of two, -inf where a position takes no part
     float x[NP];
     float mt = -INFINITY;
@@ -351,7 +433,7 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
       }
     if (more) load_v(next);
     cur = next;
-    if (t + 2 * NW < rg.t1) next = find(t + 2 * NW);
+    if (t + 2 * NW < t1) next = find(t + 2 * NW);
   }
   l = quad_sum(l);
 
@@ -374,7 +456,8 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
   }
   __syncthreads();
   const int64_t row0 = (int64_t)seq * a.num_q + head0;
-  const bool whole = rg.splits <= 1;
+  const bool whole = wk.splits <= 1;
+  const int64_t slots = (int64_t)a.num_seqs * a.s_max;
   for (int e = threadIdx.x; e < G * (HD / 4); e += NW * 64) {
     const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
     Joined<T> j;
@@ -389,49 +472,50 @@ __global__ __launch_bounds__(NW * 64, HD == 512 ? 1 : 3) void k_paged_attn(
     if (whole) {
       j.store(a, row0 + h, HD, col);
     } else {
-      const int64_t at = (row0 + h) * a.s_max + split;
+      const int64_t at = (head0 + h) * slots + wk.slot0 + wk.split;
       store_agent(a.ws_acc + at * HD + col, j.acc[0], j.acc[1]);
       store_agent(a.ws_acc + at * HD + col + 2, j.acc[2], j.acc[3]);
       if (col == 0) store_agent(a.ws_ml + at * kMlStride, M, j.L);
     }
   }
+  if (!a.tag && a.s_max > 1 && kvh == 0 && hg == 0 && wk.split == 0 && threadIdx.x == 0)
+    *plan_of(a, seq) = int2{wk.slot0, wk.splits};
   if (whole || !a.tag) return;
 
   // the splits are joined by whoever comes last
   stores_done();
-  uint64_t* marks = reinterpret_cast<uint64_t*>(a.ws_ml + row0 * a.s_max * kMlStride + 2);
-  if (!last_of(marks, kMlStride / 2, rg.splits, split, a.tag,
+  uint64_t* marks = reinterpret_cast<uint64_t*>(a.ws_ml + (head0 * slots + wk.slot0) * kMlStride + 2);
+  if (!last_of(marks, kMlStride / 2, wk.splits, wk.split, a.tag,
                reinterpret_cast<int*>(sm + 2 * NW * 16)))
     return;
-  // Maxima and sums to LDS, over the waves' parts (kJoinBytes: there are at most 192 of
-  // them, and room for 2 NW (HD + 8) at least); then eight splits' sums at a time.
-  static_assert(kJoinBytes / (4 * HD) <= NW * LD / 2 + NW * 16, "room for the splits' m and l");
-  for (int e = threadIdx.x; e < G * rg.splits; e += NW * 64) {
-    const int h = e / rg.splits, i = e - h * rg.splits;
-    const v2f v = load2_agent(a.ws_ml + ((row0 + h) * a.s_max + i) * kMlStride);
+  // Maxima and sums to LDS, over the waves' parts; then eight splits' sums at a time.
+  static_assert(2 * kJoinMost <= NW * LD, "room for the splits' m and l of each head");
+  for (int e = threadIdx.x; e < G * wk.splits; e += NW * 64) {
+    const int h = e / wk.splits, i = e - h * wk.splits;
+    const v2f v = load2_agent(a.ws_ml + ((head0 + h) * slots + wk.slot0 + i) * kMlStride);
     part[2 * e] = v[0];
     part[2 * e + 1] = v[1];
   }
   __syncthreads();
   for (int e = threadIdx.x; e < G * (HD / 4); e += NW * 64) {
     const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
-    const float* ml = part + 2 * h * rg.splits;
-    const float* acc = a.ws_acc + (row0 + h) * a.s_max * HD + col;
+    const float* ml = part + 2 * h * wk.splits;
+    const float* acc = a.ws_acc + ((head0 + h) * slots + wk.slot0) * HD + col;
     Joined<T> j;
     float M = -INFINITY;
-    for (int i = 0; i < rg.splits; ++i) M = fmaxf(M, ml[2 * i]);
+    for (int i = 0; i < wk.splits; ++i) M = fmaxf(M, ml[2 * i]);
     j.start(M);
-    for (int i0 = 0; i0 < rg.splits; i0 += 8) {
+    for (int i0 = 0; i0 < wk.splits; i0 += 8) {
       v2f lo[8], hi[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i0 + i < rg.splits) {
+        if (i0 + i < wk.splits) {
           lo[i] = load2_agent(acc + (int64_t)(i0 + i) * HD);
           hi[i] = load2_agent(acc + (int64_t)(i0 + i) * HD + 2);
         }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i0 + i < rg.splits)
+        if (i0 + i < wk.splits)
           j.add(ml[2 * (i0 + i)], ml[2 * (i0 + i) + 1], v4f32{lo[i][0], lo[i][1], hi[i][0], hi[i][1]});
     }
     j.store(a, row0 + h, HD, col);
@@ -445,10 +529,12 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a) {
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   if (row >= (int64_t)a.num_seqs * a.num_q) return;
   const int seq = (int)(row / a.num_q), col = (threadIdx.x % TPR) * 4;
-  const int S = attn_range(a, seq, 0, tile_positions<HD>()).splits;
+  const int2 plan = *plan_of(a, seq);
+  const int S = plan.y;
   if (S <= 1) return;
-  const float* ml = a.ws_ml + row * a.s_max * kMlStride;
-  const float* acc = a.ws_acc + row * a.s_max * HD + col;
+  const int64_t at = row % a.num_q * ((int64_t)a.num_seqs * a.s_max) + plan.x;
+  const float* ml = a.ws_ml + at * kMlStride;
+  const float* acc = a.ws_acc + at * HD + col;
   Joined<T> j;
   float M = -INFINITY;
   for (int s = 0; s < S; ++s) M = fmaxf(M, ml[s * kMlStride]);
@@ -464,7 +550,8 @@ template <typename T, int HD, bool SMALL>
 hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t st) {
   constexpr int NW = 4;
   const int G = std::min(16, a.gqa);
-  int64_t blocks = (int64_t)a.num_seqs * a.num_kv * a.s_max;
+  const bool up = attn_rounds_up(a.num_seqs, a.units);  // fills no more than the units
+  int64_t blocks = (up ? a.units : (int64_t)a.num_seqs * a.s_max) * a.num_kv;
   if (a.head_groups > 1) blocks = (blocks + 7) / 8 * 8 * a.head_groups;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const size_t lds = ((size_t)NW * G * (HD + 8) + 2 * NW * 16 + 4 + (queries_in_lds<HD>() ? HD * 8 : 0)) *
@@ -480,13 +567,11 @@ hipError_t launch_attn(const PagedAttnArgs& a, hipStream_t st) {
 }
 
 template <typename T, int HD>
-hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
-  constexpr int TP = tile_positions<HD>();
-  // a window that does not start on a tile reaches into one more
-  const int len = a.window > 0 ? std::min(a.window, max_len) : max_len;
-  const int64_t tiles = ((int64_t)len + TP - 1) / TP + (a.window > 0 ? 1 : 0);
-  a.chunk_tiles = (int)std::max<int64_t>(1, (tiles + a.s_max - 1) / a.s_max);
-  const bool fused = a.s_max > 1 && (int64_t)a.s_max * std::min(16, a.gqa) * HD * 4 <= kJoinBytes;
+hipError_t launch(PagedAttnArgs a, hipStream_t st) {
+  const int64_t row_bytes = (int64_t)std::min(16, a.gqa) * HD * 4;  // of a split's sums
+  a.units = attn_units(a.num_seqs, a.s_max);
+  const bool fused = a.s_max > 1 && a.units / a.num_seqs * row_bytes <= kJoinBytes;
+  a.n_max = fused ? (int)std::min<int64_t>(kJoinMost, 2 * kJoinBytes / row_bytes) : 256;
   a.tag = fused ? launch_tag() : 0;
   const hipError_t e =
       a.page_shift < 4 ? launch_attn<T, HD, true>(a, st) : launch_attn<T, HD, false>(a, st);
@@ -499,12 +584,12 @@ hipError_t launch(PagedAttnArgs a, int max_len, hipStream_t st) {
 }
 
 template <typename T>
-hipError_t launch_hd(const PagedAttnArgs& a, int hd, int max_len, hipStream_t st) {
+hipError_t launch_hd(const PagedAttnArgs& a, int hd, hipStream_t st) {
   switch (hd) {
-    case 64: return launch<T, 64>(a, max_len, st);
-    case 128: return launch<T, 128>(a, max_len, st);
-    case 256: return launch<T, 256>(a, max_len, st);
-    default: return launch<T, 512>(a, max_len, st);
+    case 64: return launch<T, 64>(a, st);
+    case 128: return launch<T, 128>(a, st);
+    case 256: return launch<T, 256>(a, st);
+    default: return launch<T, 512>(a, st);
   }
 }
 
@@ -513,23 +598,34 @@ hipError_t launch_hd(const PagedAttnArgs& a, int hd, int max_len, hipStream_t st
 // A workgroup (4 waves, a tile each at a time) per compute unit reads at the full rate
 // and leaves the fewest sums to join: 8 sequences of 16384 positions, 8 kv heads of 128:
 // 4 splits 104 us, 12 splits 105, 2 splits 137; 16 of 8000 with 32 query heads on one
-// kv head: 8 splits 20, 24 splits 26.  A few more than that run beside each other,
-// except for heads of 512, of which a unit holds one workgroup.  No split has fewer than
-// six tiles, and a sequence of three rounds has one (7 of 333 positions: 6.7, 3 splits
-// 7.2 us).
+// kv head: 8 splits 20, 24 splits 26.  Rounds of them should leave few units idle (8 kv
+// heads of 128, 500 to 8000 positions: 12 sequences, 2 workgroups for each 38 us, 3 46; 20
+// sequences: 1 110, 2 95, 3 81).  Where there are enough without splits, one for each, on
+// average, evens out lengths; heads of 256 take two (64 of up to 8192, 4 kv heads: 257 us,
+// two 223, equal lengths 349 and 364; heads of 128, 32 of up to 4096: 50 and 49, equal
+// lengths 96 and 103).  Short ones do not need it (256 of 1000, one kv head of 128: 24,
+// shared out 27).  A sequence of three rounds has one split (7 of 333 positions: 6.7, 3
+// splits 7.2 us).
 int paged_attn_splits(int num_seqs, int num_q, int num_kv, int head_dim, int max_kv_len, int window) {
   const int tp = head_dim >= 256 ? 16 : 32;
   const int64_t len = window > 0 ? std::min(max_kv_len, window) : max_kv_len;
   const int64_t tiles = (len + tp - 1) / tp + (window > 0 ? 1 : 0);
   const int64_t groups = (int64_t)num_seqs * num_kv * ((num_q / num_kv + 15) / 16);
-  const int64_t cus = tune().cus, s = head_dim == 512 ? cus / groups : (cus + groups - 1) / groups;
+  const int64_t cus = tune().cus;
   if (tiles <= 12) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({s, (tiles + 5) / 6, 256}));
+  int64_t s;
+  if (groups >= cus) {
+    if (num_seqs == 1 || num_seqs > 1024 || tiles <= 48) return 1;
+    s = head_dim == 256 ? 2 : 1;
+  } else {
+    s = cus / groups;
+    while (10 * s * groups < 7 * cus * ((s * groups + cus - 1) / cus)) ++s;
+  }
+  return (int)std::min<int64_t>({s, (tiles + 5) / 6, 255}) + (num_seqs > 1);
 }
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, int max_len, bool f16,
-                             hipStream_t st) {
-  return f16 ? launch_hd<F16>(a, head_dim, max_len, st) : launch_hd<Bf16>(a, head_dim, max_len, st);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int head_dim, bool f16, hipStream_t st) {
+  return f16 ? launch_hd<F16>(a, head_dim, st) : launch_hd<Bf16>(a, head_dim, st);
 }
 
 }  // namespace bq

@@ -38,6 +38,27 @@ BQ_HD int32_t page_number(int32_t base, int shift, int32_t num_pages) {
   return (base >> shift) < num_pages ? base >> shift : -1;
 }
 
+// The attention shares its num_seqs s_max slots per kv head out by length: a sequence
+// gets `share` of a workgroup for each of its tiles, rounded up or down (`round`), and
+// one at least; none takes fewer than kMinTiles tiles.  Rounded down, shares of
+// units / all tiles fill at most units + num_seqs - 1 slots (units, of one sequence);
+// rounded up, shares of (units - num_seqs) / all tiles fill at most units.
+constexpr int kMinTiles = 6;
+BQ_HD int attn_units(int num_seqs, int s_max) {
+  return num_seqs > 1 ? num_seqs * (s_max - 1) : s_max;
+}
+// whether the largest share that rounded up fits the units is looked for
+BQ_HD bool attn_rounds_up(int num_seqs, int units) {
+  return num_seqs > 1 && num_seqs <= 64 && units > num_seqs;
+}
+// 1e-6: the product of whole numbers may be a little off
+constexpr double kRoundDown = 1e-6, kRoundUp = 1.0 - 1e-6;
+BQ_HD int attn_splits(int tiles, double share, double round, int most) {
+  const double n = (double)tiles * share + round;
+  const int whole = n < most ? (int)n : most, room = tiles / kMinTiles;
+  return whole < 1 || room < 1 ? 1 : whole < room ? whole : room;
+}
+
 // How sequence i goes on after a reorder, from its parent's length: `full`
 // whole pages that are shared, then pages [full, end) that are its own (the
 // first of them may hold len % page_rows positions already).

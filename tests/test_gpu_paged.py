@@ -202,6 +202,28 @@ def test_paged_attention(gpu, lens, nq, nkv, hd, window, cap, dt, shift, splits)
     check_attn(gpu, *c, nq, nkv, hd, shift, window, cap, max_kv_len=max(max(lens), 1), s_max=splits)
 
 
+@pytest.mark.parametrize("lens,nq,nkv,hd,window,dt,shift,splits", [
+    ([6000] + [40] * 9, 8, 2, 128, 0, BF, 4, 2),          # 9 shares of one, joined by its last workgroup
+    ([6000] + [40] * 9, 16, 1, 128, 0, HF, 3, 4),         # capped: 16 heads' sums
+    ([3, 0, 4000, 0, 700], 8, 2, 64, 0, HF, 5, 7),
+    ([3000, 100, 1], 4, 2, 512, 0, BF, 4, 30),            # joined by a launch
+    ([2500, 33, 1200], 32, 1, 256, 2000, BF, 6, 9),       # two groups of heads, a launch
+    ([50] * 70 + [2000] + [0] * 60, 2, 1, 64, 0, BF, 0, 2),  # more sequences than lanes
+    ([0] * 130, 2, 2, 128, 0, HF, 4, 3),
+    ([200 + 9 * i for i in range(67)], 2, 2, 128, 0, BF, 4, None),
+    ([10000], 4, 1, 128, 0, BF, 4, 256),
+    ([64, 5000], 16, 1, 512, 0, HF, 4, 256),
+])
+def test_attention_unequal_lengths(gpu, lens, nq, nkv, hd, window, dt, shift, splits):
+    """Slots are shared out by length, whatever the longest sequence was said to have; the share
+    does not depend on where a sequence stands."""
+    c = attn_case(lens, nq, nkv, hd, dt, shift)
+    out = check_attn(gpu, *c, nq, nkv, hd, shift, window, 0.0, max_kv_len=max(max(lens), 1), s_max=splits)
+    q, kc, vc, table, n = (t.flip(0) if i in (0, 3, 4) else t for i, t in enumerate(c))
+    back = check_attn(gpu, q, kc, vc, table, n, nq, nkv, hd, shift, window, 0.0, max_kv_len=max(max(lens), 1), s_max=splits)
+    assert same_bits(out.flip(0), back)
+
+
 def test_attention_longer_than_planned(gpu):
     """max_kv_len only sizes the splits; None plans for the whole table."""
     c = attn_case([700, 3], 4, 2, 128, BF, 4)

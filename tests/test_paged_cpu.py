@@ -51,7 +51,7 @@ def test_rope_refusals(L):
 
 def attn(L, **kw):
     a = dict(q=P, qs=1024, kc=P, vc=P, slots=512, rows=P, width=8, shift=4, lens=P, out=P, lse=None, n=4, nq=8, nkv=4,
-             hd=128, win=0, scale=1.0, cap=0.0, dt=BF16, longest=100, s_max=2, ws=P, bytes=1 << 30, st=None)
+             hd=128, win=0, scale=1.0, cap=0.0, dt=BF16, s_max=2, ws=P, bytes=1 << 30, st=None)
     assert set(kw) <= set(a)
     a.update(kw)
     return L.bq_paged_attention(*a.values())
@@ -64,7 +64,7 @@ def test_attention_refusals(L):
     assert attn(L, dt=F32) == 1 and attn(L, dt=77) == 1
     for name in ("q", "kc", "vc", "out", "ws"):
         assert attn(L, **{name: C.c_void_p(264)}) == 1, name
-    for kw in (dict(hd=80), dict(nq=7), dict(nkv=0), dict(width=0), dict(win=-1), dict(longest=-1), dict(s_max=0),
+    for kw in (dict(hd=80), dict(nq=7), dict(nkv=0), dict(width=0), dict(win=-1), dict(s_max=0),
                dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("nan")), dict(qs=1023), dict(qs=1000),
                dict(bytes=4 * 8 * 2 * 132 * 4 - 1), dict(slots=-1), dict(slots=0)):
         assert attn(L, **kw) == 2, kw
@@ -195,6 +195,62 @@ int main() {
   }
 }
 """
+
+
+SHARES = r"""
+#include <stdio.h>
+#include "bq_pages.hpp"
+int main() {
+  int n, s_max, most;
+  while (scanf("%d %d %d", &n, &s_max, &most) == 3) {
+    static int tiles[1024];
+    double sum = 0.0;
+    for (int i = 0; i < n; ++i) scanf("%d", tiles + i), sum += tiles[i];
+    const int units = bq::attn_units(n, s_max);
+    const double share = sum > 0.0 ? units / sum : 0.0;
+    for (int i = 0; i < n; ++i) printf("%d ", bq::attn_splits(tiles[i], share, bq::kRoundDown, most));
+    int up = 0;
+    for (int i = 0; i < n; ++i)
+      up += bq::attn_splits(tiles[i], sum > 0.0 ? (units - n) / sum : 0.0, bq::kRoundUp, most);
+    printf("%d\n", units < n || up <= units);
+  }
+}
+"""
+
+
+def test_attention_shares(tmp_path):
+    """Slots shared out by length: never more than there are, at least one each, as many as asked
+    for where all are alike, most of them to the one that is long."""
+    if not shutil.which("g++"):
+        pytest.skip("no host compiler")
+    src, exe = tmp_path / "shares.cpp", tmp_path / "shares"
+    src.write_text(SHARES)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wno-unused-result", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-I", os.path.join(ROOT, "mojo-gemma4-cpu_amd", "csrc"), str(src), "-o",
+                    str(exe)], check=True)
+    rng, cases = random.Random(6), []
+    for _ in range(2000):
+        n, s_max, most = rng.choice([1, 2, 3, 17, 64, 65, 300]), rng.choice([2, 3, 9, 33, 256]), rng.choice([6, 128, 256])
+        top = rng.choice([0, 5, 40, 3000, 2**27])
+        tiles = [rng.randint(0, top) for _ in range(n)]
+        if rng.random() < 0.3:
+            tiles = [top] * n
+        if rng.random() < 0.3:
+            tiles[rng.randrange(n)] = 2**27
+        cases.append((s_max, most, tiles))
+    text = "\n".join(f"{len(t)} {s} {m} " + " ".join(map(str, t)) for s, m, t in cases)
+    got = subprocess.run([str(exe)], input=text, text=True, capture_output=True, check=True).stdout.splitlines()
+    assert len(got) == len(cases)
+    for (s_max, most, tiles), line in zip(cases, got):
+        *n, fits = (int(v) for v in line.split())
+        assert fits  # where a search for the largest share that fits begins
+        assert len(n) == len(tiles) and sum(n) <= len(n) * s_max
+        assert all(1 <= v <= max(1, min(most, t // 6)) for v, t in zip(n, tiles))
+        each = s_max if len(n) == 1 else s_max - 1
+        if len(set(tiles)) == 1:
+            assert set(n) == {max(1, min(each, most, tiles[0] // 6))}
+        if sorted(tiles)[-1] == 2**27 and sum(tiles) < 2**27 + 2**20:
+            assert max(n) >= min(most, int(each * len(n) * 0.99))
 
 
 def test_page_arithmetic(tmp_path):
